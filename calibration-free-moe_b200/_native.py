@@ -14,20 +14,20 @@ import subprocess
 from pathlib import Path
 
 PACKAGE = Path(__file__).resolve().parent
-SOURCES = [PACKAGE / "csrc" / "cfm_reader.cu"]
+SOURCES = [PACKAGE / "csrc" / "cfm_reader.cu", PACKAGE / "csrc" / "cfm_logits.cu"]
 HEADERS = [PACKAGE / "csrc" / "cfm_device.cuh", PACKAGE / "csrc" / "cfm_union.cuh",
            PACKAGE / "csrc" / "cfm_exchange.cuh", PACKAGE / "csrc" / "cfm_select.cuh",
            PACKAGE / "csrc" / "cfm_build.cuh", PACKAGE / "csrc" / "cfm_screen.cuh",
            PACKAGE / "csrc" / "cfm_screen_tc.cuh", PACKAGE / "csrc" / "cfm_prepare.cuh",
-           PACKAGE / "csrc" / "cfm_rules.cuh",
+           PACKAGE / "csrc" / "cfm_rules.cuh", PACKAGE / "csrc" / "cfm_launch.cuh",
            PACKAGE.parent / "include" / "cfm_b200.h"]
 LIBRARY = PACKAGE / "libcfm_b200.so"
-ABI_VERSION = 12
+ABI_VERSION = 13
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
     "-lineinfo", "-O3", "-std=c++17",
-    "-shared", "-Xcompiler", "-fPIC",
+    "-shared", "-Xcompiler", "-fPIC", "--threads", "0",
 ]
 
 # Entry points include/cfm_b200.h declares; `load()` checks each one resolves.
@@ -37,8 +37,9 @@ STAGES = (
 )
 PEER_SYMBOLS = ("cfm_build_sketch", "cfm_exchange_bytes", "cfm_peer_alloc", "cfm_peer_export", "cfm_peer_import",
                 "cfm_peer_release", "cfm_exchange_status", "cfm_finish_rows")
+LOGITS_SYMBOLS = ("cfm_route_tokens", "cfm_token_logprobs", "cfm_compare_logits")
 SYMBOLS = (("cfm_abi_version", "cfm_error_string", "cfm_workspace_layout_for", "cfm_finish")
-           + STAGES + PEER_SYMBOLS)
+           + STAGES + PEER_SYMBOLS + LOGITS_SYMBOLS)
 MAX_RANKS = 16
 PEER_HANDLE_BYTES = 64
 
@@ -106,6 +107,19 @@ class Exchange(ctypes.Structure):
         ("tokens", ctypes.c_int32),
         ("reserved", ctypes.c_int32),
         ("blocks", ctypes.c_void_p * MAX_RANKS),
+    ]
+
+
+class Rows(ctypes.Structure):
+    """`struct cfm_rows`."""
+
+    _fields_ = [
+        ("data", ctypes.c_void_p),
+        ("stride", ctypes.c_int64),
+        ("rows", ctypes.c_int32),
+        ("columns", ctypes.c_int32),
+        ("type", ctypes.c_int32),
+        ("reserved", ctypes.c_int32),
     ]
 
 
@@ -220,6 +234,14 @@ def load() -> ctypes.CDLL:
         ctypes.POINTER(Layer), ctypes.POINTER(Exchange), ctypes.c_void_p, ctypes.c_void_p,
         ctypes.c_void_p,
     ]
+    rows, pointer, number = ctypes.POINTER(Rows), ctypes.c_void_p, ctypes.c_int32
+    library.cfm_route_tokens.argtypes = [rows, number, number, pointer, number, pointer, number, pointer]
+    library.cfm_token_logprobs.argtypes = [
+        rows, pointer, number, number, pointer, pointer, pointer, pointer, pointer,
+    ]
+    library.cfm_compare_logits.argtypes = [rows, rows, pointer, pointer, pointer]
+    for symbol in LOGITS_SYMBOLS:
+        getattr(library, symbol).restype = ctypes.c_int
     _library = library
     return library
 

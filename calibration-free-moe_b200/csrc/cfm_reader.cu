@@ -17,6 +17,7 @@
 // launch shape.  No kernel waits on another: cross-CTA reductions use the
 // "last CTA to arrive finishes" pattern with an atomic counter and no spin.
 #include "cfm_device.cuh"
+#include "cfm_launch.cuh"
 
 #include "cfm_b200.h"
 
@@ -2080,35 +2081,6 @@ static int bind_call(const cfm_layer* layer, void* workspace, int32_t capacity,
   // Without a row-major sketch that the expert-major screen can read, the coordinate-major one is.
   if (screened && !layer->sketch && !screens_grouped(*b)) return CFM_E_NULL;
   return 0;
-}
-
-// Launch with programmatic stream serialisation: the kernel may be scheduled while its
-// predecessor in the stream is finishing and waits for it at grid_dependency_wait().
-// Used for every launch of a whole call (measured for two of them: 0.6 to 1.3 us per call).  CFM_PDL=0 in the environment makes these ordinary
-// launches.
-template <typename... Params, typename... Args>
-static void launch_dependent(void (*kernel)(Params...), dim3 grid, dim3 block, size_t smem,
-                             cudaStream_t stream, Args... args) {
-  static const bool on = [] {
-    const char* v = std::getenv("CFM_PDL");
-    return !v || std::atoi(v) != 0;
-  }();
-  cudaLaunchConfig_t config = {};
-  config.gridDim = grid;
-  config.blockDim = block;
-  config.dynamicSmemBytes = smem;
-  config.stream = stream;
-  cudaLaunchAttribute attribute[1];
-  attribute[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attribute[0].val.programmaticStreamSerializationAllowed = 1;
-  config.attrs = attribute;
-  config.numAttrs = on ? 1 : 0;
-  (void)cudaLaunchKernelEx(&config, kernel, static_cast<Params>(args)...);
-}
-
-static int launched() {
-  const cudaError_t err = cudaGetLastError();
-  return err == cudaSuccess ? 0 : static_cast<int>(err);
 }
 
 // Layers that have a row-major sketch screen expert-major (the kernels read it 16 bytes at a time).

@@ -30,7 +30,7 @@
 extern "C" {
 #endif
 
-#define CFM_ABI_VERSION 12
+#define CFM_ABI_VERSION 13
 
 /* argument errors */
 #define CFM_E_NULL -1       /* a required pointer is NULL                      */
@@ -404,6 +404,52 @@ typedef struct cfm_static_screen {
  * No counterpart in the reference, whose scratch is always caller-allocated
  * (ReaderWorkspace). */
 int cfm_screen_static(const cfm_layer* layer, const cfm_static_screen* io, void* stream);
+
+/* ---- the exact side of a decode step --------------------------------------- */
+/* Router, whole routed experts and scores of logits: what a decode step has around the
+ * reader, and what the reader's output is held against.  Like the stages above these
+ * enqueue their work on the caller's stream, allocate nothing, never synchronise and can be
+ * captured.  They are for inference: no gradients.  No counterpart in the reference, which
+ * leaves these to the engine and to torch (runtime/experts.py:1275-1288,
+ * eval/fidelity.py:34-48). */
+#define CFM_TYPE_BF16 0
+#define CFM_TYPE_F16 1
+#define CFM_TYPE_F32 2
+
+/* Rows of a matrix on the device, each contiguous, `stride` elements apart; data at the
+ * alignment of an element.  No rows is a call without work. */
+typedef struct cfm_rows {
+  const void* data;
+  int64_t stride;
+  int32_t rows;
+  int32_t columns;
+  int32_t type;           /* CFM_TYPE_*                                        */
+  int32_t reserved;
+} cfm_rows;
+
+/* Router: of every row of E <= 1024 logits the top_k <= 32 largest, in descending order,
+ * equal ones by the lowest index, NaN above all; their softmax probabilities over the row, or with
+ * `renormalize` over the experts picked.  `ids` int32 or int64 [T, K], `weights` FP32 or
+ * BF16 [T, K]: what cfm_route and cfm_experts_forward take. */
+int cfm_route_tokens(const cfm_rows* logits, int32_t top_k, int32_t renormalize, void* ids,
+                     int32_t ids_are_int64, void* weights, int32_t weights_are_bf16, void* stream);
+
+/* Scores of rows of V <= 2^21 logits: the log probability of each row's given token (NaN for
+ * a token outside of the row), the entropy of the row's distribution in nats, and the `top`
+ * <= 32 largest logits in the router's order: `top_ids` int32 and `top_logprobs` FP32
+ * [T, top], not touched with `top` 0.  `tokens` int32 or int64 [T].  An element of -inf has no
+ * probability.  A row of nothing but -inf, with NaN or with +inf has no distribution: its
+ * numbers are NaN, its top ids in order all the same. */
+int cfm_token_logprobs(const cfm_rows* logits, const void* tokens, int32_t tokens_are_int64,
+                       int32_t top, float* logprobs, float* entropy, int32_t* top_ids,
+                       float* top_logprobs, void* stream);
+
+/* Two sets of rows of one shape and type: KL(softmax(reference) || softmax(logits)) of each
+ * pair in nats, and whether the largest logits are at the same place (ties as above).  +inf
+ * where the reference gives weight to what the other gives none; NaN where either has no
+ * distribution. */
+int cfm_compare_logits(const cfm_rows* reference, const cfm_rows* logits, float* divergence,
+                       uint8_t* agreement, void* stream);
 
 #ifdef __cplusplus
 }
