@@ -14,7 +14,8 @@ import subprocess
 from pathlib import Path
 
 PACKAGE = Path(__file__).resolve().parent
-SOURCES = [PACKAGE / "csrc" / "cfm_reader.cu", PACKAGE / "csrc" / "cfm_logits.cu"]
+SOURCES = [PACKAGE / "csrc" / "cfm_reader.cu", PACKAGE / "csrc" / "cfm_logits.cu",
+           PACKAGE / "csrc" / "cfm_experts.cu"]
 HEADERS = [PACKAGE / "csrc" / "cfm_device.cuh", PACKAGE / "csrc" / "cfm_union.cuh",
            PACKAGE / "csrc" / "cfm_exchange.cuh", PACKAGE / "csrc" / "cfm_select.cuh",
            PACKAGE / "csrc" / "cfm_build.cuh", PACKAGE / "csrc" / "cfm_screen.cuh",
@@ -38,8 +39,9 @@ STAGES = (
 PEER_SYMBOLS = ("cfm_build_sketch", "cfm_exchange_bytes", "cfm_peer_alloc", "cfm_peer_export", "cfm_peer_import",
                 "cfm_peer_release", "cfm_exchange_status", "cfm_finish_rows")
 LOGITS_SYMBOLS = ("cfm_route_tokens", "cfm_token_logprobs", "cfm_compare_logits")
+EXPERTS_SYMBOLS = ("cfm_experts_workspace_bytes", "cfm_experts_forward")
 SYMBOLS = (("cfm_abi_version", "cfm_error_string", "cfm_workspace_layout_for", "cfm_finish")
-           + STAGES + PEER_SYMBOLS + LOGITS_SYMBOLS)
+           + STAGES + PEER_SYMBOLS + LOGITS_SYMBOLS + EXPERTS_SYMBOLS)
 MAX_RANKS = 16
 PEER_HANDLE_BYTES = 64
 
@@ -120,6 +122,21 @@ class Rows(ctypes.Structure):
         ("columns", ctypes.c_int32),
         ("type", ctypes.c_int32),
         ("reserved", ctypes.c_int32),
+    ]
+
+
+class Experts(ctypes.Structure):
+    """`struct cfm_experts`."""
+
+    _fields_ = [
+        ("hidden", ctypes.c_int32),
+        ("width", ctypes.c_int32),
+        ("experts", ctypes.c_int32),
+        ("top_k", ctypes.c_int32),
+        ("activation", ctypes.c_int32),
+        ("reserved", ctypes.c_int32),
+        ("gate_up", ctypes.c_void_p),
+        ("down", ctypes.c_void_p),
     ]
 
 
@@ -242,6 +259,12 @@ def load() -> ctypes.CDLL:
     library.cfm_compare_logits.argtypes = [rows, rows, pointer, pointer, pointer]
     for symbol in LOGITS_SYMBOLS:
         getattr(library, symbol).restype = ctypes.c_int
+    library.cfm_experts_workspace_bytes.restype = ctypes.c_int64
+    library.cfm_experts_workspace_bytes.argtypes = [ctypes.POINTER(Experts), number]
+    library.cfm_experts_forward.restype = ctypes.c_int
+    library.cfm_experts_forward.argtypes = [
+        ctypes.POINTER(Experts), pointer, number, ctypes.POINTER(Call), pointer,
+    ]
     _library = library
     return library
 
