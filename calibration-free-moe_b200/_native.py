@@ -21,6 +21,7 @@ HEADERS = [PACKAGE / "csrc" / "cfm_device.cuh", PACKAGE / "csrc" / "cfm_union.cu
            PACKAGE / "csrc" / "cfm_build.cuh", PACKAGE / "csrc" / "cfm_screen.cuh",
            PACKAGE / "csrc" / "cfm_screen_tc.cuh", PACKAGE / "csrc" / "cfm_prepare.cuh",
            PACKAGE / "csrc" / "cfm_rules.cuh", PACKAGE / "csrc" / "cfm_launch.cuh",
+           PACKAGE / "csrc" / "cfm_tc.cuh", PACKAGE / "csrc" / "cfm_experts_tc.cuh",
            PACKAGE.parent / "include" / "cfm_b200.h"]
 LIBRARY = PACKAGE / "libcfm_b200.so"
 ABI_VERSION = 13

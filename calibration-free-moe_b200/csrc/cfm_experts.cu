@@ -4,24 +4,32 @@
 // A call is bound by the weights of the experts that some token is routed to, so the (token, slot) pairs are
 // grouped by expert and each weight is read once for all tokens of its expert:
 //   group   counts, offsets and the list of pairs by expert
-//   up      gate and up rows, activation, BF16 [pair, I] in the order of the list
+//   up      gate and up rows, activation, two BF16 terms [pair, I]
 //   down    channel-major down rows, FP32 [pair, H]
 //   mix     router weights, sum over a token's slots in their order, BF16
-// Sums are FP32; the activations are rounded to BF16 once, for the tensor cores take the type of the weights.
-// A pair's numbers do not depend on its place in the list nor on the other pairs, so neither does a token's
-// output on the tokens beside it.
+// Sums are FP32.  The tensor cores take the type of the weights, so an activation goes to them as two BF16
+// terms, its value rounded and what that leaves: 2^-17 of it is lost, and of the output's error of 2^-9 nothing is theirs.
+// (Rounded once to BF16 they would have added as much as the output's own rounding: 0.0024 of the output's norm
+// instead of 0.0016.)
+// A pair's numbers do not depend on its place in the list nor on the other pairs: a token's output does not depend
+// on the tokens beside it, but for calls of few pairs, whose kernels add in another order.
 #include "cfm_device.cuh"
 #include "cfm_launch.cuh"
+#include "cfm_tc.cuh"
 
 #include "cfm_b200.h"
 
+#include <cuda.h>
+
 #include <algorithm>
+#include <type_traits>
 
 namespace cfm {
 namespace {
 
 constexpr int kMaxExperts = 4096;
-constexpr int kMaxWidth = 8192;  // eight tokens' activations fit shared memory
+constexpr int kLeastPass = 16;    // pairs that the smallest pass of the tensor-core path takes
+constexpr int kMaxWidth = 4096;  // eight tokens' activations fit shared memory
 
 struct Experts {
   int H, I, E, K, activation;
@@ -33,8 +41,11 @@ struct Scratch {
   int32_t* offsets;  // [E + 1] first pair of every expert
   int32_t* pairs;    // [C K] pairs by expert
   int32_t* busy;     // [E] experts that have pairs
-  int32_t* counts;   // [4] number of those
+  int4* passes;      // expert, first pair, pairs: of the tensor-core path
+  int32_t* counts;   // [4] number of busy experts, of passes
+  int32_t* status;   // [4] device-side errors
   __nv_bfloat16* activations;  // [C K, I]
+  __nv_bfloat16* rests;        // [C K, I] what the activations' rounding leaves
   float* sums;                 // [C K, H]
 };
 
@@ -62,6 +73,13 @@ __device__ __forceinline__ float gated(float g, float u, int activation) {
   return __fdividef(g, 1.0f + __expf(-z)) * u;
 }
 
+__device__ __forceinline__ void store_activation(const Scratch& s, size_t at, float a) {
+  const __nv_bfloat16 rounded = __float2bfloat16_rn(a);
+  const float value = __bfloat162float(rounded);
+  s.activations[at] = rounded;
+  s.rests[at] = __float2bfloat16_rn(fabsf(value) < __builtin_huge_valf() ? a - value : 0.0f);  // of inf and NaN nothing
+}
+
 __device__ __forceinline__ void mma_bf16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
                                          uint32_t b0, uint32_t b1) {
   asm volatile(
@@ -74,7 +92,8 @@ __device__ __forceinline__ void mma_bf16(float (&c)[4], uint32_t a0, uint32_t a1
 // ---- group: one CTA --------------------------------------------------------------------------------
 constexpr int kGroupThreads = 1024;
 
-__global__ void __launch_bounds__(kGroupThreads) k_group_pairs(Routes routes, int E, int K, Scratch s) {
+// `tokens`: pairs of a pass.
+__global__ void __launch_bounds__(kGroupThreads) k_group_pairs(Routes routes, int E, int K, int tokens, Scratch s) {
   extern __shared__ int group_shared[];
   __shared__ int scan[33];
   int* count = group_shared;  // [E], then the next place of every expert
@@ -90,24 +109,28 @@ __global__ void __launch_bounds__(kGroupThreads) k_group_pairs(Routes routes, in
   __syncthreads();
   // Offsets, and the experts that have pairs, in order.
   const int per = (E + kGroupThreads - 1) / kGroupThreads, from = min(E, tid * per), to = min(E, from + per);
-  int mine = 0, busy = 0;
+  int mine = 0, busy = 0, parts = 0;
   for (int e = from; e < to; ++e) {
     mine += count[e];
     busy += count[e] > 0;
+    parts += (count[e] + tokens - 1) / tokens;
   }
-  int total, experts;
+  int total, experts, passes;
   int offset = block_exclusive_scan(mine, scan, &total);
   int place = block_exclusive_scan(busy, scan, &experts);
+  int part = block_exclusive_scan(parts, scan, &passes);
   for (int e = from; e < to; ++e) {
     const int n = count[e];
     s.offsets[e] = offset;
     count[e] = offset;
+    for (int at = 0; at < n; at += tokens) s.passes[part++] = make_int4(e, offset + at, min(tokens, n - at), 0);
     offset += n;
     if (n) s.busy[place++] = e;
   }
   if (tid == 0) {
     s.offsets[E] = total;
     s.counts[0] = experts;
+    s.counts[1] = passes;
   }
   __syncthreads();
   for (int p = tid; p < pairs; p += kGroupThreads) {
@@ -214,8 +237,8 @@ __global__ void __launch_bounds__(kThreads, 2)
         for (int j = 1; j < kSplits; ++j) sum += of[j * TILES * 128];
         gu[half] = sum;
       }
-      s.activations[static_cast<size_t>(first + pass + token) * L.I + c0 + c] =
-          __float2bfloat16_rn(gated(gu[0], gu[1], L.activation));
+      store_activation(s, static_cast<size_t>(s.pairs[first + pass + token]) * L.I + c0 + c,
+                       gated(gu[0], gu[1], L.activation));
     }
     __syncthreads();
   }
@@ -255,8 +278,9 @@ __global__ void __launch_bounds__(kThreads, 2) k_experts_down(Experts L, Scratch
     __syncthreads();
     for (int i = tid; i < tokens * (L.I / 8); i += kThreads) {
       const int row = i / (L.I / 8), piece = i - row * (L.I / 8);
-      copy_async16(shared_u32(down_shared + row * stride + 16 * piece),
-                   s.activations + static_cast<size_t>(first + pass + row) * L.I + 8 * piece);
+      const size_t from = static_cast<size_t>(s.pairs[first + pass + row]) * L.I + 8 * piece;
+      copy_async16(shared_u32(down_shared + row * stride + 16 * piece), s.activations + from);
+      copy_async16(shared_u32(down_shared + (kTokens + row) * stride + 16 * piece), s.rests + from);
     }
     copy_async_commit();
     copy_async_wait<0>();
@@ -280,10 +304,15 @@ __global__ void __launch_bounds__(kThreads, 2) k_experts_down(Experts L, Scratch
         if (step + kDownAhead < end) fetch(w[i], step + kDownAhead);
 #pragma unroll
         for (int n = 0; n < TILES; ++n) {
-          uint32_t b0, b1;
-          asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(b0), "=r"(b1) : "r"(x + n * 8 * stride + 32 * step));
 #pragma unroll
-          for (int j = 0; j < 4; ++j) mma_bf16(acc[n][j], a[j][0], a[j][1], a[j][2], a[j][3], b0, b1);
+          for (int term = 0; term < 2; ++term) {
+            uint32_t b0, b1;
+            asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];"
+                         : "=r"(b0), "=r"(b1)
+                         : "r"(x + (term * kTokens + n * 8) * stride + 32 * step));
+#pragma unroll
+            for (int j = 0; j < 4; ++j) mma_bf16(acc[n][j], a[j][0], a[j][1], a[j][2], a[j][3], b0, b1);
+          }
         }
       }
     }
@@ -316,9 +345,11 @@ __global__ void __launch_bounds__(kThreads, 2) k_experts_down(Experts L, Scratch
 
 template <int TILES>
 static size_t down_shared_bytes(int I) {
-  const size_t rows = 8 * TILES * static_cast<size_t>((2 * I + 127) / 128 * 128 + 32);
+  const size_t rows = 2 * 8 * TILES * static_cast<size_t>((2 * I + 127) / 128 * 128 + 32);
   return std::max(rows, static_cast<size_t>(kThreads / 32) * 8 * TILES * 64 * sizeof(float));
 }
+
+#include "cfm_experts_tc.cuh"
 
 // ---- mix -------------------------------------------------------------------------------------------
 constexpr int kMixThreads = 128;
@@ -373,11 +404,14 @@ int64_t lay_out(const cfm_experts* x, int64_t capacity, void* base, Scratch* s) 
   Scratch none;
   Scratch* to = s ? s : &none;
   const int64_t pairs = capacity * x->top_k;
+  take(&to->status, 4);
   take(&to->offsets, x->experts + 1);
   take(&to->pairs, pairs);
   take(&to->busy, x->experts);
+  take(&to->passes, std::min<int64_t>(x->experts, pairs) + pairs / kLeastPass);
   take(&to->counts, 4);
   take(&to->activations, pairs * x->width);
+  take(&to->rests, pairs * x->width);
   take(&to->sums, pairs * x->hidden);
   return at;
 }
@@ -396,6 +430,45 @@ int run_tiles(const Experts& L, const Scratch& s, const __nv_bfloat16* hidden, i
   if (code) return code;
   launch_dependent(k_experts_up<TILES>, dim3(L.I / kUpChannels, busy), dim3(kThreads), Up<TILES>::kBytes, stream, L, s, hidden);
   launch_dependent(k_experts_down<TILES>, dim3(L.H / kDownColumns, busy), dim3(kThreads), down, stream, L, s);
+  return 0;
+}
+
+// The map of a matrix [rows, columns] in boxes of 64 columns and 64 rows, swizzled by 128 bytes.
+int make_map(CUtensorMap* map, const void* data, int64_t rows, int64_t columns) {
+  static const auto encode = [] {
+    void* found = nullptr;
+    cudaDriverEntryPointQueryResult result;
+    if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &found, 12000, cudaEnableDefault, &result) != cudaSuccess ||
+        result != cudaDriverEntryPointSuccess)
+      found = nullptr;
+    return reinterpret_cast<decltype(&cuTensorMapEncodeTiled)>(found);
+  }();
+  if (!encode) return static_cast<int>(cudaErrorNotSupported);
+  const cuuint64_t sizes[2] = {static_cast<cuuint64_t>(columns), static_cast<cuuint64_t>(rows)};
+  const cuuint64_t strides[1] = {static_cast<cuuint64_t>(columns) * 2};
+  const cuuint32_t box[2] = {kTensorColumns, 64}, steps[2] = {1, 1};
+  const CUresult code = encode(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(data), sizes, strides, box, steps,
+                               CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return code == CUDA_SUCCESS ? 0 : static_cast<int>(cudaErrorInvalidValue);
+}
+
+template <int TOKENS>
+int run_tensor(const Experts& L, const Scratch& s, const __nv_bfloat16* hidden, int64_t pairs, cudaStream_t stream) {
+  using U = Tensor<TOKENS, false>;
+  using D = Tensor<TOKENS, true>;
+  CUtensorMap up, down;
+  int code = make_map(&up, L.gate_up, static_cast<int64_t>(L.E) * 2 * L.I, L.H);
+  if (!code) code = make_map(&down, L.down, static_cast<int64_t>(L.E) * L.I, L.H);
+  if (!code) code = allow_shared(k_experts_tensor<TOKENS, false>, U::kShared);
+  if (!code) code = allow_shared(k_experts_tensor<TOKENS, true>, D::kShared);
+  if (code) return code;
+  const int64_t passes = std::min<int64_t>(L.E, pairs) + pairs / TOKENS;
+  const auto ctas = [&](int tiles) { return dim3(static_cast<unsigned>(std::min<int64_t>(148, passes * tiles))); };
+  launch_dependent(k_experts_tensor<TOKENS, false>, ctas((L.I + kUpTile - 1) / kUpTile), dim3(kTensorThreads), U::kShared,
+                   stream, L, s, hidden, up);
+  launch_dependent(k_experts_tensor<TOKENS, true>, ctas(L.H / kTensorRows), dim3(kTensorThreads), D::kShared, stream, L, s,
+                   hidden, down);
   return 0;
 }
 
@@ -428,10 +501,13 @@ int cfm_experts_forward(const cfm_experts* layer, void* workspace, int32_t capac
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
   const int64_t pairs = static_cast<int64_t>(L.K) * call->tokens;
   const int busy = static_cast<int>(std::min<int64_t>(L.E, pairs));
-  launch_dependent(k_group_pairs, dim3(1), dim3(kGroupThreads), sizeof(int) * L.E, st, routes, L.E, L.K, s);
-  const int code = pairs > 8 * L.E ? run_tiles<4>(L, s, hidden, busy, st)
-                   : pairs > 4 * L.E ? run_tiles<2>(L, s, hidden, busy, st)
-                                     : run_tiles<1>(L, s, hidden, busy, st);
+  const int pass = pairs <= 8 * busy ? 16 : pairs <= 20 * busy ? 32 : pairs <= 48 * busy ? 64 : 128;
+  launch_dependent(k_group_pairs, dim3(1), dim3(kGroupThreads), sizeof(int) * L.E, st, routes, L.E, L.K, pass, s);
+  const int code = pairs <= 32    ? run_tiles<1>(L, s, hidden, busy, st)
+                   : pass == 16   ? run_tensor<16>(L, s, hidden, pairs, st)
+                   : pass == 32   ? run_tensor<32>(L, s, hidden, pairs, st)
+                   : pass == 64   ? run_tensor<64>(L, s, hidden, pairs, st)
+                                  : run_tensor<128>(L, s, hidden, pairs, st);
   if (code) return code;
   launch_dependent(k_experts_mix, dim3(call->tokens, (L.H + 8 * kMixThreads - 1) / (8 * kMixThreads)), dim3(kMixThreads), 0,
                    st, L, s, routes, static_cast<__nv_bfloat16*>(call->out));

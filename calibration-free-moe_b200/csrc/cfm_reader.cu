@@ -18,6 +18,7 @@
 // "last CTA to arrive finishes" pattern with an atomic counter and no spin.
 #include "cfm_device.cuh"
 #include "cfm_launch.cuh"
+#include "cfm_tc.cuh"
 
 #include "cfm_b200.h"
 

@@ -32,7 +32,8 @@ class RoutedWorkspace:
         self.bytes = _native.load().cfm_experts_workspace_bytes(ctypes.byref(layer), capacity)
         if self.bytes < 0:
             raise ValueError(_native.load().cfm_error_string(self.bytes).decode())
-        self.buffer = torch.empty(self.bytes, device=device, dtype=torch.uint8)
+        self.buffer = torch.zeros(self.bytes, device=device, dtype=torch.uint8)
+        self.status = self.buffer[:4].view(torch.int32)
 
 
 class RoutedExperts:
@@ -40,7 +41,7 @@ class RoutedExperts:
 
     gate_up BF16 `[E, 2I, H]` (gate rows, then up rows), contiguous; down BF16, logical `[E, H, I]`
     in the storage of `channel_major_down`: what `ProgressiveReader` takes, and the two may share
-    them.  H a multiple of 128, I of 16, E up to 4096, top_k up to 32.  Calls take up to
+    them.  H a multiple of 128, I of 16 up to 4096, E up to 4096, top_k up to 32.  Calls take up to
     `max_tokens` tokens.  Inference only.
     """
 
@@ -164,6 +165,12 @@ class RoutedExperts:
                              ctypes.byref(call), torch._C._cuda_getCurrentRawStream(index))
         if code:
             _native.check(code, "cfm_experts_forward")
+
+    def check_status(self) -> None:
+        """Raise if a wait inside a kernel of this workspace's calls ran out (they end after a
+        second); that call's rows are not to be trusted.  Synchronises with the device."""
+        if int(self.workspace.status):
+            raise RuntimeError("routed-expert kernels reported a device-side error")
 
     def rows(self, x: Tensor, topk_weights: Tensor, topk_ids: Tensor) -> Tensor:
         """Any number of rows, in calls of at most `max_tokens`: the stock callable of

@@ -454,7 +454,7 @@ int cfm_compare_logits(const cfm_rows* reference, const cfm_rows* logits, float*
 /* The routed experts of a layer as a whole: dimensions and weights, as in cfm_layer. */
 typedef struct cfm_experts {
   int32_t hidden;         /* H, multiple of 128, at most 65536                 */
-  int32_t width;          /* I, multiple of 16, at most 8192                   */
+  int32_t width;          /* I, multiple of 16, at most 4096                   */
   int32_t experts;        /* E <= 4096                                         */
   int32_t top_k;          /* K <= 32                                           */
   int32_t activation;     /* CFM_ACT_*                                         */
@@ -464,14 +464,17 @@ typedef struct cfm_experts {
 } cfm_experts;
 
 /* Scratch bytes for calls of up to `capacity` tokens (a host computation; negative: a CFM_E_*
- * code).  The scratch needs no initialisation; one call at a time may use it. */
+ * code).  The caller zeroes the scratch once; one call at a time may use it.  Its first int32 is
+ * a status: not zero if a wait inside a kernel ran out (after about a second), when the
+ * outputs of that call are not to be trusted. */
 int64_t cfm_experts_workspace_bytes(const cfm_experts* layer, int32_t capacity);
 
 /* out[t] = sum over slots k of weights[t, k] D_e (phi(G_e x_t) * (U_e x_t)), e = ids[t, k], all
  * channels.  Of `call`: tokens, ids, weights, padding, hidden, out and the two type flags, as
- * cfm_reader_forward takes them.  An id outside of [0, E) adds nothing; a token may have an expert
- * more than once.  Padding rows read nothing and produce zero rows.  Sums are FP32, the activations
- * rounded to BF16 once, the output once. */
+ * cfm_reader_forward takes them; hidden, out and the weights on 16-byte boundaries.  An id outside of [0, E) adds nothing; a token may have an expert
+ * more than once.  Padding rows read nothing and produce zero rows.  Sums are FP32, activations keep
+ * 16 bits, the output is rounded once.  A token's bits do not depend on the other tokens, except
+ * between calls of up to 32 (token, slot) pairs and larger ones. */
 int cfm_experts_forward(const cfm_experts* layer, void* workspace, int32_t capacity,
                         const cfm_call* call, void* stream);
 
