@@ -28,7 +28,7 @@ namespace cfm {
 namespace {
 
 constexpr int kMaxExperts = 4096;
-constexpr int kLeastPass = 16;    // pairs that the smallest pass of the tensor-core path takes
+constexpr int kLeastPass = 32;    // pairs that the smallest pass of the tensor-core path takes
 constexpr int kMaxWidth = 4096;  // eight tokens' activations fit shared memory
 
 struct Experts {
@@ -40,6 +40,7 @@ struct Experts {
 struct Scratch {
   int32_t* offsets;  // [E + 1] first pair of every expert
   int32_t* pairs;    // [C K] pairs by expert
+  int32_t* tokens;   // [C K] their tokens
   int32_t* busy;     // [E] experts that have pairs
   int4* passes;      // expert, first pair, pairs: of the tensor-core path
   int32_t* counts;   // [4] number of busy experts, of passes
@@ -90,35 +91,65 @@ __device__ __forceinline__ void mma_bf16(float (&c)[4], uint32_t a0, uint32_t a1
 }
 
 // ---- group: one CTA --------------------------------------------------------------------------------
+// All latency (9 us of a call of 64 tokens when every pair was looked at twice and three sums were scanned): a
+// thread keeps its pairs' experts and their places among the expert's pairs, which one pass of atomics gives,
+// and the three sums are scanned as one number.  The order of an expert's pairs is as it comes.
 constexpr int kGroupThreads = 1024;
+constexpr int kGroupKept = 8;  // pairs of a thread that stay in registers; of larger calls the rest is looked at twice
+constexpr int64_t kMostPairs = 1 << 24;
 
 // `tokens`: pairs of a pass.
 __global__ void __launch_bounds__(kGroupThreads) k_group_pairs(Routes routes, int E, int K, int tokens, Scratch s) {
   extern __shared__ int group_shared[];
-  __shared__ int scan[33];
-  int* count = group_shared;  // [E], then the next place of every expert
-  const int tid = threadIdx.x, pairs = routes.tokens * K;
+  __shared__ uint64_t warps[32];
+  int* count = group_shared;  // [E], then the first place of every expert
+  const int tid = threadIdx.x, lane = tid & 31, pairs = routes.tokens * K;
   for (int e = tid; e < E; e += kGroupThreads) count[e] = 0;
   __syncthreads();
   grid_dependency_wait();
   grid_dependency_release();
-  for (int p = tid; p < pairs; p += kGroupThreads) {
+  int expert[kGroupKept], rank[kGroupKept];
+#pragma unroll
+  for (int j = 0; j < kGroupKept; ++j) {
+    const int p = tid + j * kGroupThreads;
+    expert[j] = p < pairs ? routes.expert(p, K, E) : -1;
+  }
+#pragma unroll
+  for (int j = 0; j < kGroupKept; ++j)
+    if (expert[j] >= 0) rank[j] = atomicAdd(&count[expert[j]], 1);
+  for (int p = tid + kGroupKept * kGroupThreads; p < pairs; p += kGroupThreads) {
     const int e = routes.expert(p, K, E);
     if (e >= 0) atomicAdd(&count[e], 1);
   }
   __syncthreads();
-  // Offsets, and the experts that have pairs, in order.
+  // Pairs, passes and busy experts before those of this thread, in one number.
+  constexpr int kPassBits = 24, kBusyBits = kPassBits + 22;
   const int per = (E + kGroupThreads - 1) / kGroupThreads, from = min(E, tid * per), to = min(E, from + per);
-  int mine = 0, busy = 0, parts = 0;
-  for (int e = from; e < to; ++e) {
-    mine += count[e];
-    busy += count[e] > 0;
-    parts += (count[e] + tokens - 1) / tokens;
+  uint64_t mine = 0;
+  for (int e = from; e < to; ++e)
+    if (const int n = count[e])
+      mine += static_cast<uint64_t>(n) | static_cast<uint64_t>((n + tokens - 1) / tokens) << kPassBits | 1ull << kBusyBits;
+  uint64_t sum = mine;
+#pragma unroll
+  for (int w = 1; w < 32; w <<= 1) {
+    const uint64_t other = __shfl_up_sync(kFull, sum, w);
+    if (lane >= w) sum += other;
   }
-  int total, experts, passes;
-  int offset = block_exclusive_scan(mine, scan, &total);
-  int place = block_exclusive_scan(busy, scan, &experts);
-  int part = block_exclusive_scan(parts, scan, &passes);
+  if (lane == 31) warps[tid >> 5] = sum;
+  __syncthreads();
+  if (tid < 32) {
+    uint64_t all = warps[tid];
+#pragma unroll
+    for (int w = 1; w < 32; w <<= 1) {
+      const uint64_t other = __shfl_up_sync(kFull, all, w);
+      if (lane >= w) all += other;
+    }
+    warps[tid] = all;
+  }
+  __syncthreads();
+  const uint64_t before = sum - mine + (tid >= 32 ? warps[(tid >> 5) - 1] : 0), all = warps[31];
+  int offset = static_cast<int>(before & ((1u << kPassBits) - 1)), part = static_cast<int>(before >> kPassBits & ((1u << 22) - 1));
+  int place = static_cast<int>(before >> kBusyBits);
   for (int e = from; e < to; ++e) {
     const int n = count[e];
     s.offsets[e] = offset;
@@ -128,14 +159,31 @@ __global__ void __launch_bounds__(kGroupThreads) k_group_pairs(Routes routes, in
     if (n) s.busy[place++] = e;
   }
   if (tid == 0) {
-    s.offsets[E] = total;
-    s.counts[0] = experts;
-    s.counts[1] = passes;
+    s.offsets[E] = static_cast<int>(all & ((1u << kPassBits) - 1));
+    s.counts[0] = static_cast<int>(all >> kBusyBits);
+    s.counts[1] = static_cast<int>(all >> kPassBits & ((1u << 22) - 1));
   }
   __syncthreads();
-  for (int p = tid; p < pairs; p += kGroupThreads) {
+#pragma unroll
+  for (int j = 0; j < kGroupKept; ++j) {
+    if (expert[j] < 0) continue;
+    const int p = tid + j * kGroupThreads, at = count[expert[j]] + rank[j];
+    s.pairs[at] = p;
+    s.tokens[at] = p / K;
+  }
+  if (pairs <= kGroupKept * kGroupThreads) return;
+  // The other pairs come behind those.
+  __syncthreads();
+#pragma unroll
+  for (int j = 0; j < kGroupKept; ++j)
+    if (expert[j] >= 0) atomicAdd(&count[expert[j]], 1);
+  __syncthreads();
+  for (int p = tid + kGroupKept * kGroupThreads; p < pairs; p += kGroupThreads) {
     const int e = routes.expert(p, K, E);
-    if (e >= 0) s.pairs[atomicAdd(&count[e], 1)] = p;
+    if (e < 0) continue;
+    const int at = atomicAdd(&count[e], 1);
+    s.pairs[at] = p;
+    s.tokens[at] = p / K;
   }
 }
 
@@ -191,7 +239,7 @@ __global__ void __launch_bounds__(kThreads, 2)
       __syncthreads();  // the columns before have been read
       for (int i = tid; i < tokens * (columns / 8); i += kThreads) {
         const int row = i / (columns / 8), piece = i - row * (columns / 8);
-        const int token = s.pairs[first + pass + row] / L.K;
+        const int token = s.tokens[first + pass + row];
         copy_async16(shared_u32(up_shared + row * U::kStride + 16 * piece),
                      hidden + static_cast<size_t>(token) * L.H + k0 + 8 * piece);
       }
@@ -407,6 +455,7 @@ int64_t lay_out(const cfm_experts* x, int64_t capacity, void* base, Scratch* s) 
   take(&to->status, 4);
   take(&to->offsets, x->experts + 1);
   take(&to->pairs, pairs);
+  take(&to->tokens, pairs);
   take(&to->busy, x->experts);
   take(&to->passes, std::min<int64_t>(x->experts, pairs) + pairs / kLeastPass);
   take(&to->counts, 4);
@@ -453,6 +502,14 @@ int make_map(CUtensorMap* map, const void* data, int64_t rows, int64_t columns) 
   return code == CUDA_SUCCESS ? 0 : static_cast<int>(cudaErrorInvalidValue);
 }
 
+// Pairs of a pass, for `busy` experts.  A second pass over an expert reads its weights again, from L2; a stage with room for more
+// tokens leaves fewer stages in the ring.  Passes of 16, 32, 64, 128 (and 192), us of a call: 64 tokens of the
+// 128-expert layer (4 per expert) 200, 195, 196, 205; 256 of 256 experts with a skewed router (8) 192, 168, 168, 169;
+// 1000 of 64 experts (125) 828, 452, 299, 234, 216.
+int pass_pairs(int64_t pairs, int64_t busy) {
+  return pairs <= 12 * busy ? 32 : pairs <= 32 * busy ? 64 : pairs <= 80 * busy ? 128 : 192;
+}
+
 template <int TOKENS>
 int run_tensor(const Experts& L, const Scratch& s, const __nv_bfloat16* hidden, int64_t pairs, cudaStream_t stream) {
   using U = Tensor<TOKENS, false>;
@@ -465,9 +522,9 @@ int run_tensor(const Experts& L, const Scratch& s, const __nv_bfloat16* hidden, 
   if (code) return code;
   const int64_t passes = std::min<int64_t>(L.E, pairs) + pairs / TOKENS;
   const auto ctas = [&](int tiles) { return dim3(static_cast<unsigned>(std::min<int64_t>(148, passes * tiles))); };
-  launch_dependent(k_experts_tensor<TOKENS, false>, ctas((L.I + kUpTile - 1) / kUpTile), dim3(kTensorThreads), U::kShared,
+  launch_dependent(k_experts_tensor<TOKENS, false>, ctas((L.I + kUpTile - 1) / kUpTile), dim3(U::kThreads), U::kShared,
                    stream, L, s, hidden, up);
-  launch_dependent(k_experts_tensor<TOKENS, true>, ctas(L.H / kTensorRows), dim3(kTensorThreads), D::kShared, stream, L, s,
+  launch_dependent(k_experts_tensor<TOKENS, true>, ctas(L.H / kTensorRows), dim3(D::kThreads), D::kShared, stream, L, s,
                    hidden, down);
   return 0;
 }
@@ -482,7 +539,7 @@ extern "C" {
 int64_t cfm_experts_workspace_bytes(const cfm_experts* layer, int32_t capacity) {
   const int code = check_experts(layer);
   if (code) return code;
-  if (capacity < 1 || static_cast<int64_t>(capacity) * layer->top_k > (1 << 28)) return CFM_E_CAPACITY;
+  if (capacity < 1 || static_cast<int64_t>(capacity) * layer->top_k >= kMostPairs) return CFM_E_CAPACITY;
   return lay_out(layer, capacity, nullptr, nullptr);
 }
 
@@ -501,13 +558,13 @@ int cfm_experts_forward(const cfm_experts* layer, void* workspace, int32_t capac
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
   const int64_t pairs = static_cast<int64_t>(L.K) * call->tokens;
   const int busy = static_cast<int>(std::min<int64_t>(L.E, pairs));
-  const int pass = pairs <= 8 * busy ? 16 : pairs <= 20 * busy ? 32 : pairs <= 48 * busy ? 64 : 128;
+  const int pass = pass_pairs(pairs, busy);
   launch_dependent(k_group_pairs, dim3(1), dim3(kGroupThreads), sizeof(int) * L.E, st, routes, L.E, L.K, pass, s);
   const int code = pairs <= 32    ? run_tiles<1>(L, s, hidden, busy, st)
-                   : pass == 16   ? run_tensor<16>(L, s, hidden, pairs, st)
                    : pass == 32   ? run_tensor<32>(L, s, hidden, pairs, st)
                    : pass == 64   ? run_tensor<64>(L, s, hidden, pairs, st)
-                                  : run_tensor<128>(L, s, hidden, pairs, st);
+                   : pass == 128  ? run_tensor<128>(L, s, hidden, pairs, st)
+                                  : run_tensor<192>(L, s, hidden, pairs, st);
   if (code) return code;
   launch_dependent(k_experts_mix, dim3(call->tokens, (L.H + 8 * kMixThreads - 1) / (8 * kMixThreads)), dim3(kMixThreads), 0,
                    st, L, s, routes, static_cast<__nv_bfloat16*>(call->out));

@@ -7,7 +7,7 @@
 //
 //   * one thread of warp 4 brings weights by TMA into a ring of 16-KB stages in shared memory, across the
 //     borders of the items: the ring is what hides the latency of HBM;
-//   * warps 6 and 7 bring the tokens' columns of the same stages, rows gathered with cp.async;
+//   * the warps from 6 on bring the tokens' columns of the same stages, rows gathered with cp.async;
 //   * one thread of warp 5 issues the products, into one of two places in tensor memory;
 //   * warps 0 to 3 turn the sums of the item before into results meanwhile.
 //
@@ -18,25 +18,26 @@
 // Included by cfm_experts.cu inside its namespace.
 #pragma once
 
-constexpr int kTensorThreads = 256;
 constexpr int kTensorRows = 128;     // of weights, M
 constexpr int kTensorColumns = 64;   // k of a stage: rows of 128 bytes, swizzled by 16-byte pieces
 constexpr int kUpTile = 64;          // channels of an item
-constexpr int kGatherThreads = 64;
 
 template <int TOKENS, bool DOWN>
 struct Tensor {
+  // Threads that gather tokens.  64 tokens of the 128-expert layer in passes of 16: 198 us with 64 of them, 201 with
+  // 128; 1000 tokens of 64 experts in passes of 128: 274 with 64, 237 with 128.
+  static constexpr int kGatherThreads = TOKENS <= 32 ? 64 : 128;
+  static constexpr int kGatherRows = kGatherThreads / 8;  // a row of a stage is eight pieces
+  static constexpr int kThreads = 192 + kGatherThreads;
   static constexpr int kWeightBytes = kTensorRows * 128;
   static constexpr int kTermBytes = TOKENS * 128;
   static constexpr int kStage = kWeightBytes + kTermBytes * (DOWN ? 2 : 1);
   static constexpr int kExchange = DOWN ? 0 : 2 * 4 * 8 * 32 * 4;  // two blocks of four warps' eight columns
   static constexpr int kRoom = 227 * 1024 - 1024 - 1024 - kExchange;  // less alignment and barriers
   static constexpr int kStages = kRoom / kStage < 12 ? kRoom / kStage : 12;
-  static constexpr int kLag = kStages / 2;  // stages whose tokens are on their way
-  static constexpr int kPlace = TOKENS < 16 ? 16 : TOKENS;         // columns of tensor memory of one of two places
+  static constexpr int kPlace = TOKENS > 128 ? 256 : TOKENS;  // columns of tensor memory of one of two places
   static constexpr uint32_t kTensorMemory = 2 * kPlace < 32 ? 32 : 2 * kPlace;
   static constexpr size_t kShared = 1024 + static_cast<size_t>(kStages) * kStage + kExchange;
-  static_assert(kStages >= 3 && kLag < kStages && kLag >= 1, "the tokens' copies never wait for themselves");
   static_assert((kTensorMemory & (kTensorMemory - 1)) == 0 && kTensorMemory <= 512, "a power of two");
 };
 
@@ -75,6 +76,11 @@ __device__ __forceinline__ void copy_box(uint32_t shared, const CUtensorMap* map
       : "memory");
 }
 
+// Arrives at the barrier once the thread's cp.async copies so far have landed.
+__device__ __forceinline__ void copies_arrive(uint32_t bar) {
+  asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory");
+}
+
 // All of the four result warps, once all have come: whether every one of them is alive.
 __device__ __forceinline__ bool result_warps_agree(int alive) {
   uint32_t all;
@@ -94,7 +100,7 @@ __device__ __forceinline__ void result_warps_meet() { asm volatile("barrier.cta.
 
 // grid: at most one CTA per SM.  `weights`: the map of the weight with boxes of 64 columns and 64 rows.
 template <int TOKENS, bool DOWN>
-__global__ void __launch_bounds__(kTensorThreads, 1)
+__global__ void __launch_bounds__(Tensor<TOKENS, DOWN>::kThreads, 1)
     k_experts_tensor(Experts L, Scratch s, const __nv_bfloat16* hidden, const __grid_constant__ CUtensorMap weights) {
   using S = Tensor<TOKENS, DOWN>;
   using namespace tc;
@@ -115,7 +121,7 @@ __global__ void __launch_bounds__(kTensorThreads, 1)
     abort_flag = late_flag = s_filled = 0;
     for (int i = 0; i < S::kStages; ++i) {
       barrier_init(weights_in + 8 * i, 1);
-      barrier_init(tokens_in + 8 * i, kGatherThreads / 32);
+      barrier_init(tokens_in + 8 * i, S::kGatherThreads);
       barrier_init(freed + 8 * i, 1);
     }
     for (int i = 0; i < 2; ++i) {
@@ -147,15 +153,19 @@ __global__ void __launch_bounds__(kTensorThreads, 1)
   const int tiles = DOWN ? H / kTensorRows : (I + kUpTile - 1) / kUpTile;
   const int chunks = DOWN ? (I + kTensorColumns - 1) / kTensorColumns : H / kTensorColumns;
   const int items = __ldcg(&s.counts[1]) * tiles;
-  auto pass_of = [&](int item) { return __ldcg(&s.passes[item / tiles]); };  // expert, first, count
+  // Expert, first pair, pairs.  Each role asks for an item's pass while it is at the item before.
+  auto pass_of = [&](int item) { return item < items ? __ldcg(&s.passes[item / tiles]) : make_int4(0, 0, 0, 0); };
+  const int step = gridDim.x;
 
   if (warp == 4) {
     // ---- weights ----
     if (elect_lane()) {
       int alive = 1, filled = 0, stage = 0;
       uint32_t turn = 1;  // parity of the round before; the first round finds all stages free
-      for (int item = blockIdx.x; item < items && alive; item += gridDim.x) {
-        const int e = pass_of(item).x, tile = item % tiles;
+      int4 next = pass_of(blockIdx.x);
+      for (int item = blockIdx.x; item < items && alive; item += step) {
+        const int e = next.x, tile = item % tiles;
+        next = pass_of(item + step);
         for (int c = 0; c < chunks; ++c) {
           const uint32_t bar = weights_in + 8 * stage, to = ring + stage * S::kStage;
           if (filled >= S::kStages) {
@@ -187,8 +197,10 @@ __global__ void __launch_bounds__(kTensorThreads, 1)
     if (elect_lane()) {
       int alive = 1, stage = 0, round = 0;
       uint32_t turn = 0;
-      for (int item = blockIdx.x; item < items && alive; item += gridDim.x, ++round) {
-        const int count = pass_of(item).z, place = round & 1;
+      int4 next = pass_of(blockIdx.x);
+      for (int item = blockIdx.x; item < items && alive; item += step, ++round) {
+        const int count = next.z, place = round & 1;
+        next = pass_of(item + step);
         const uint32_t sums = tmem + place * S::kPlace, what = instruction((count + 15) / 16 * 16, DOWN);
         if (round >= 2) barrier_wait(taken + 8 * place, ((round >> 1) - 1) & 1, abort, alive);
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
@@ -196,6 +208,7 @@ __global__ void __launch_bounds__(kTensorThreads, 1)
           barrier_wait(weights_in + 8 * stage, turn, abort, alive);
           barrier_wait(tokens_in + 8 * stage, turn, abort, alive);
           if (!alive) break;
+          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // the tokens came by ordinary copies
           asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
           const uint32_t from = ring + stage * S::kStage;
           const uint64_t a = descriptor(from, DOWN), b = descriptor(from + S::kWeightBytes, false);
@@ -224,25 +237,28 @@ __global__ void __launch_bounds__(kTensorThreads, 1)
       grid_dependency_wait();
       grid_dependency_release();
     }
-    const int at = tid - (kTensorThreads - kGatherThreads), row0 = at >> 3, piece = at & 7;
+    const int at = tid - 192, row0 = at >> 3, piece = at & 7;
     const uint32_t place = row0 * 128 + ((piece ^ (row0 & 7)) << 4);
-    int alive = 1, filled = 0, stage = 0, told = 0;
+    constexpr int kRows = (TOKENS + S::kGatherRows - 1) / S::kGatherRows;
+    const int32_t* list = DOWN ? s.pairs : s.tokens;
+    int alive = 1, filled = 0, stage = 0;
     uint32_t turn = 1;
-    auto tell = [&] {  // the oldest stage that has not been told of
-      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-      __syncwarp();
-      barrier_arrive(tokens_in + 8 * told, lane == 0);
-      told = told + 1 == S::kStages ? 0 : told + 1;
-    };
-    for (int item = blockIdx.x; item < items && alive; item += gridDim.x) {
-      const int4 pass = pass_of(item);
-      int row[TOKENS / 8];
+    // Rows are asked for an item ahead, passes two.
+    int row[kRows], next_row[kRows];
+    auto rows_of = [&](const int4& pass) {
 #pragma unroll
-      for (int j = 0; j < TOKENS / 8; ++j) {
-        const int t = row0 + 8 * j;
-        const int pair = t < pass.z ? __ldcg(&s.pairs[pass.y + t]) : -1;
-        row[j] = DOWN || pair < 0 ? pair : pair / L.K;
+      for (int j = 0; j < kRows; ++j) {
+        const int t = row0 + S::kGatherRows * j;
+        next_row[j] = t < pass.z ? __ldcg(&list[pass.y + t]) : -1;
       }
+    };
+    rows_of(pass_of(blockIdx.x));
+    int4 next = pass_of(blockIdx.x + step);
+    for (int item = blockIdx.x; item < items && alive; item += step) {
+#pragma unroll
+      for (int j = 0; j < kRows; ++j) row[j] = next_row[j];
+      rows_of(next);
+      next = pass_of(item + 2 * step);
       for (int c = 0; c < chunks; ++c) {
         if (filled >= S::kStages) barrier_wait(freed + 8 * stage, turn, abort, alive);
         if (!__all_sync(kFull, alive)) {
@@ -253,22 +269,18 @@ __global__ void __launch_bounds__(kTensorThreads, 1)
         const int column = c * kTensorColumns + 8 * piece;
         if (!DOWN || column < I) {
 #pragma unroll
-          for (int j = 0; j < TOKENS / 8; ++j) {
+          for (int j = 0; j < kRows; ++j) {
             if (row[j] < 0) continue;
             if (DOWN) {
               const size_t from = static_cast<size_t>(row[j]) * I + column;
-              copy_async16(to + j * 1024, s.activations + from);
-              copy_async16(to + S::kTermBytes + j * 1024, s.rests + from);
+              copy_async16(to + j * S::kGatherRows * 128, s.activations + from);
+              copy_async16(to + S::kTermBytes + j * S::kGatherRows * 128, s.rests + from);
             } else {
-              copy_async16(to + j * 1024, hidden + static_cast<size_t>(row[j]) * H + column);
+              copy_async16(to + j * S::kGatherRows * 128, hidden + static_cast<size_t>(row[j]) * H + column);
             }
           }
         }
-        copy_async_commit();
-        if (filled >= S::kLag) {
-          copy_async_wait<S::kLag>();
-          tell();
-        }
+        copies_arrive(tokens_in + 8 * stage);
         ++filled;
         if (++stage == S::kStages) {
           stage = 0;
@@ -276,9 +288,7 @@ __global__ void __launch_bounds__(kTensorThreads, 1)
         }
       }
     }
-    copy_async_wait<0>();
-    if (alive)
-      for (int left = min(filled, S::kLag); left > 0; --left) tell();
+    asm volatile("cp.async.wait_all;" ::: "memory");
   } else {
     // ---- results ----
     if (DOWN) {
@@ -288,8 +298,10 @@ __global__ void __launch_bounds__(kTensorThreads, 1)
     const uint32_t lanes = static_cast<uint32_t>(warp * 32) << 16;
     float* exchange = reinterpret_cast<float*>(tensor_shared + (ring - shared_u32(tensor_shared)) + S::kStages * S::kStage);
     int alive = 1, round = 0, turn = 0;
-    for (int item = blockIdx.x; item < items; item += gridDim.x, ++round) {
-      const int4 pass = pass_of(item);
+    int4 next = pass_of(blockIdx.x);
+    for (int item = blockIdx.x; item < items; item += step, ++round) {
+      const int4 pass = next;
+      next = pass_of(item + step);
       const int count = pass.z, tile = item % tiles, place = round & 1;
       int pairs[(TOKENS + 31) / 32];
 #pragma unroll

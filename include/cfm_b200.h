@@ -463,7 +463,7 @@ typedef struct cfm_experts {
   const void* down;       /* bf16 physical [E, I, H] (channel-major)           */
 } cfm_experts;
 
-/* Scratch bytes for calls of up to `capacity` tokens (a host computation; negative: a CFM_E_*
+/* Scratch bytes for calls of up to `capacity` tokens, fewer than 2^24 pairs (a host computation; negative: a CFM_E_*
  * code).  The caller zeroes the scratch once; one call at a time may use it.  Its first int32 is
  * a status: not zero if a wait inside a kernel ran out (after about a second), when the
  * outputs of that call are not to be trusted. */
