@@ -3,10 +3,11 @@
 //
 // A call is bound by the weights of the experts that some token is routed to, so the (token, slot) pairs are
 // grouped by expert and each weight is read once for all tokens of its expert:
-//   group   counts, offsets and the list of pairs by expert
+//   group   the list of pairs by expert, and the passes over the experts
 //   up      gate and up rows, activation, two BF16 terms [pair, I]
 //   down    channel-major down rows, FP32 [pair, H]
 //   mix     router weights, sum over a token's slots in their order, BF16
+// up and down are cfm_experts_tc.cuh's; calls of few pairs have two kernels of their own, without lists.
 // Sums are FP32.  The tensor cores take the type of the weights, so an activation goes to them as two BF16
 // terms, its value rounded and what that leaves: 2^-17 of it is lost, and of the output's error of 2^-9 nothing is theirs.
 // (Rounded once to BF16 they would have added as much as the output's own rounding: 0.0024 of the output's norm
@@ -29,7 +30,6 @@ namespace {
 
 constexpr int kMaxExperts = 4096;
 constexpr int kLeastPass = 32;    // pairs that the smallest pass of the tensor-core path takes
-constexpr int kMaxWidth = 4096;  // eight tokens' activations fit shared memory
 
 struct Experts {
   int H, I, E, K, activation;
@@ -38,12 +38,10 @@ struct Experts {
 };
 
 struct Scratch {
-  int32_t* offsets;  // [E + 1] first pair of every expert
   int32_t* pairs;    // [C K] pairs by expert
   int32_t* tokens;   // [C K] their tokens
-  int32_t* busy;     // [E] experts that have pairs
   int4* passes;      // expert, first pair, pairs: of the tensor-core path
-  int32_t* counts;   // [4] number of busy experts, of passes
+  int32_t* counts;   // [4] number of passes
   int32_t* status;   // [4] device-side errors
   __nv_bfloat16* activations;  // [C K, I]
   __nv_bfloat16* rests;        // [C K, I] what the activations' rounding leaves
@@ -56,15 +54,15 @@ struct Routes {
   const uint8_t* padding;
   int tokens, ids64, weights16;
 
-  // The expert of a pair, -1 where it has none.
+  // The expert of a pair, -1 where it has none.  (From L2: a kernel may ask before its predecessor has ended.)
   __device__ int expert(int pair, int K, int E) const {
-    if (padding && padding[pair / K]) return -1;
-    const int64_t e = ids64 ? static_cast<const int64_t*>(ids)[pair] : static_cast<const int32_t*>(ids)[pair];
+    if (padding && __ldcg(&padding[pair / K])) return -1;
+    const int64_t e = ids64 ? __ldcg(&static_cast<const long long*>(ids)[pair]) : __ldcg(&static_cast<const int32_t*>(ids)[pair]);
     return e >= 0 && e < E ? static_cast<int>(e) : -1;
   }
   __device__ float weight(int pair) const {
-    return weights16 ? __bfloat162float(static_cast<const __nv_bfloat16*>(weights)[pair])
-                     : static_cast<const float*>(weights)[pair];
+    return weights16 ? __bfloat162float(__ldcg(&static_cast<const __nv_bfloat16*>(weights)[pair]))
+                     : __ldcg(&static_cast<const float*>(weights)[pair]);
   }
 };
 
@@ -93,7 +91,7 @@ __device__ __forceinline__ void mma_bf16(float (&c)[4], uint32_t a0, uint32_t a1
 // ---- group: one CTA --------------------------------------------------------------------------------
 // All latency (9 us of a call of 64 tokens when every pair was looked at twice and three sums were scanned): a
 // thread keeps its pairs' experts and their places among the expert's pairs, which one pass of atomics gives,
-// and the three sums are scanned as one number.  The order of an expert's pairs is as it comes.
+// and the two sums are scanned as one number.  The order of an expert's pairs is as it comes.
 constexpr int kGroupThreads = 1024;
 constexpr int kGroupKept = 8;  // pairs of a thread that stay in registers; of larger calls the rest is looked at twice
 constexpr int64_t kMostPairs = 1 << 24;
@@ -122,13 +120,13 @@ __global__ void __launch_bounds__(kGroupThreads) k_group_pairs(Routes routes, in
     if (e >= 0) atomicAdd(&count[e], 1);
   }
   __syncthreads();
-  // Pairs, passes and busy experts before those of this thread, in one number.
-  constexpr int kPassBits = 24, kBusyBits = kPassBits + 22;
+  // Pairs and passes before those of this thread, in one number.
+  constexpr int kPassBits = 24;
   const int per = (E + kGroupThreads - 1) / kGroupThreads, from = min(E, tid * per), to = min(E, from + per);
   uint64_t mine = 0;
   for (int e = from; e < to; ++e)
     if (const int n = count[e])
-      mine += static_cast<uint64_t>(n) | static_cast<uint64_t>((n + tokens - 1) / tokens) << kPassBits | 1ull << kBusyBits;
+      mine += static_cast<uint64_t>(n) | static_cast<uint64_t>((n + tokens - 1) / tokens) << kPassBits;
   uint64_t sum = mine;
 #pragma unroll
   for (int w = 1; w < 32; w <<= 1) {
@@ -147,22 +145,15 @@ __global__ void __launch_bounds__(kGroupThreads) k_group_pairs(Routes routes, in
     warps[tid] = all;
   }
   __syncthreads();
-  const uint64_t before = sum - mine + (tid >= 32 ? warps[(tid >> 5) - 1] : 0), all = warps[31];
-  int offset = static_cast<int>(before & ((1u << kPassBits) - 1)), part = static_cast<int>(before >> kPassBits & ((1u << 22) - 1));
-  int place = static_cast<int>(before >> kBusyBits);
+  const uint64_t before = sum - mine + (tid >= 32 ? warps[(tid >> 5) - 1] : 0);
+  int offset = static_cast<int>(before & ((1u << kPassBits) - 1)), part = static_cast<int>(before >> kPassBits);
   for (int e = from; e < to; ++e) {
     const int n = count[e];
-    s.offsets[e] = offset;
     count[e] = offset;
     for (int at = 0; at < n; at += tokens) s.passes[part++] = make_int4(e, offset + at, min(tokens, n - at), 0);
     offset += n;
-    if (n) s.busy[place++] = e;
   }
-  if (tid == 0) {
-    s.offsets[E] = static_cast<int>(all & ((1u << kPassBits) - 1));
-    s.counts[0] = static_cast<int>(all >> kBusyBits);
-    s.counts[1] = static_cast<int>(all >> kPassBits & ((1u << 22) - 1));
-  }
+  if (tid == 0) s.counts[0] = static_cast<int>(warps[31] >> kPassBits);
   __syncthreads();
 #pragma unroll
   for (int j = 0; j < kGroupKept; ++j) {
@@ -187,214 +178,195 @@ __global__ void __launch_bounds__(kGroupThreads) k_group_pairs(Routes routes, in
   }
 }
 
-// ---- up --------------------------------------------------------------------------------------------
-constexpr int kThreads = 256;
-constexpr int kSplits = 4;             // of a sum, over the warps of a CTA
-constexpr int kUpChannels = 16;        // of a CTA: two warps' tiles of eight gate and eight up rows
-constexpr int kUpAhead = 4;            // steps of 32 columns whose rows are on their way
+// ---- few pairs -------------------------------------------------------------------------------------
+// Calls of up to 32 pairs in two launches.  The weights go from global memory straight into the registers of
+// warp-level tensor-core products (m16n8k16), whose eight columns are the tokens of an expert.  Every warp
+// groups the pairs by itself, a pair per lane.
+constexpr int kFewPairs = 32;
 
-// Tokens of a pass, columns of x in shared memory at a time.
-template <int TILES>
-struct Up {
-  static constexpr int kTokens = 8 * TILES;
-  static constexpr int kColumns = 4096 / TILES;
-  static constexpr int kStride = 2 * kColumns + 64;  // bytes; rows of eight tokens fall into different banks
-  static constexpr size_t kBytes = static_cast<size_t>(kTokens) * kStride;
-  static constexpr size_t kSums = static_cast<size_t>(kThreads) * 4 * TILES * sizeof(float);
-  static_assert(kSums <= kBytes, "the sums take the place of x");
+struct Few {
+  int e;          // expert, -1: there are fewer
+  unsigned mask;  // its pairs
+  int experts;    // number of busy ones
+  bool twice;     // some token has it twice
 };
+// The `which`-th busy expert, in the order of first pairs.
+__device__ __forceinline__ Few few_pairs(const Routes& routes, int K, int E, int which) {
+  const int lane = threadIdx.x & 31;
+  const int e = lane < routes.tokens * K ? routes.expert(lane, K, E) : -1;
+  const unsigned same = __match_any_sync(kFull, e);
+  unsigned first = __ballot_sync(kFull, e >= 0 && lane == __ffs(same) - 1);
+  Few few = {-1, 0, __popc(first), false};
+  if (which >= few.experts) return few;
+  for (int i = 0; i < which; ++i) first &= first - 1;
+  const int from = __ffs(first) - 1;
+  few.e = __shfl_sync(kFull, e, from);
+  few.mask = __shfl_sync(kFull, same, from);
+  const unsigned token = __match_any_sync(kFull, lane / K);
+  few.twice = __any_sync(kFull, e == few.e && (token & few.mask & ~(1u << lane)) != 0);
+  return few;
+}
+// The pair at a place among the set bits, -1 behind them.
+__device__ __forceinline__ int pair_at(unsigned mask, int place) {
+  for (int i = 0; i < place; ++i) mask &= mask - 1;
+  return __ffs(mask) - 1;
+}
 
-// grid (I / 16, experts that can have pairs).  Weights go from global memory into the registers of the tensor
-// cores' first operand as they lie: a thread has 16 bytes of a gate row and of an up row, whose
-// elements are the k of two instructions, in an order that x is read in too.  Gate and up of a channel end in
-// one thread.
-template <int TILES>
-__global__ void __launch_bounds__(kThreads, 2)
-    k_experts_up(Experts L, Scratch s, const __nv_bfloat16* hidden) {
-  using U = Up<TILES>;
-  extern __shared__ __align__(16) uint8_t up_shared[];
+constexpr int kFewUpThreads = 128;
+constexpr int kFewUpAhead = 4;  // steps of 32 columns whose rows are on their way
+
+// grid (I / 8, experts that can have pairs).  A CTA has eight channels, its warps share the columns.  A thread
+// has 16 bytes of a gate row and of an up row, whose elements are the k of two instructions, and the same
+// of a token's row; gate and up of a channel end in one thread.
+__global__ void __launch_bounds__(kFewUpThreads, 6)
+    k_few_up(Experts L, Scratch s, Routes routes, const __nv_bfloat16* hidden) {
+  __shared__ float sums[kFewUpThreads / 32][4][32];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
   grid_dependency_wait();
   grid_dependency_release();
-  if (static_cast<int>(blockIdx.y) >= s.counts[0]) return;
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
-  const int split = warp & (kSplits - 1), tile = warp / kSplits;
-  const int e = s.busy[blockIdx.y], first = s.offsets[e], pairs = s.offsets[e + 1] - first;
-  const int c0 = blockIdx.x * kUpChannels;
-  const __nv_bfloat16* gate = L.gate_up + (static_cast<size_t>(e) * 2 * L.I + c0 + 8 * tile + g) * L.H + 8 * t;
+  const Few few = few_pairs(routes, L.K, L.E, blockIdx.y);
+  if (few.e < 0) return;
+  const int count = __popc(few.mask), c0 = 8 * blockIdx.x, steps = L.H / 128, at = 32 * warp + 8 * t;
+  const __nv_bfloat16* gate = L.gate_up + (static_cast<size_t>(few.e) * 2 * L.I + c0 + g) * L.H + at;
   const __nv_bfloat16* up = gate + static_cast<size_t>(L.I) * L.H;
-
-  for (int pass = 0; pass < pairs; pass += U::kTokens) {
-    const int tokens = min(U::kTokens, pairs - pass);
-    float acc[TILES][4] = {};
-    for (int k0 = 0; k0 < L.H; k0 += U::kColumns) {
-      const int columns = min(U::kColumns, L.H - k0), steps = columns / (32 * kSplits);
-      const size_t at = k0 + 32 * split;  // a warp's steps lie 128 columns apart, whatever the passes are
-      uint4 a[kUpAhead], b[kUpAhead];
+  for (int pass = 0; pass < count; pass += 8) {
+    const int pair = pair_at(few.mask, pass + g);
+    const __nv_bfloat16* x = hidden + static_cast<size_t>(max(pair, 0) / L.K) * L.H + at;
+    float acc[4] = {};
+    uint4 a[kFewUpAhead], b[kFewUpAhead], v[kFewUpAhead];
+    auto fetch = [&](int i, int step) {
+      a[i] = load_stream16(gate + 128 * step);
+      b[i] = load_stream16(up + 128 * step);
+      v[i] = pair >= 0 ? __ldg(reinterpret_cast<const uint4*>(x + 128 * step)) : make_uint4(0, 0, 0, 0);
+    };
 #pragma unroll
-      for (int i = 0; i < kUpAhead; ++i)
-        if (i < steps) {
-          a[i] = load_stream16(gate + at + 128 * i);
-          b[i] = load_stream16(up + at + 128 * i);
-        }
-      __syncthreads();  // the columns before have been read
-      for (int i = tid; i < tokens * (columns / 8); i += kThreads) {
-        const int row = i / (columns / 8), piece = i - row * (columns / 8);
-        const int token = s.tokens[first + pass + row];
-        copy_async16(shared_u32(up_shared + row * U::kStride + 16 * piece),
-                     hidden + static_cast<size_t>(token) * L.H + k0 + 8 * piece);
-      }
-      copy_async_commit();
-      copy_async_wait<0>();
-      __syncthreads();
-      const uint32_t x = shared_u32(up_shared) + g * U::kStride + 64 * split + 16 * t;
-      for (int from = 0; from < steps; from += kUpAhead) {
+    for (int i = 0; i < kFewUpAhead; ++i)
+      if (i < steps) fetch(i, i);
+    for (int from = 0; from < steps; from += kFewUpAhead) {
 #pragma unroll
-        for (int i = 0; i < kUpAhead; ++i) {
-          if (from + i >= steps) break;
-          const uint4 ga = a[i], ua = b[i];
-          if (from + i + kUpAhead < steps) {
-            a[i] = load_stream16(gate + at + 128 * (from + i + kUpAhead));
-            b[i] = load_stream16(up + at + 128 * (from + i + kUpAhead));
-          }
-#pragma unroll
-          for (int n = 0; n < TILES; ++n) {
-            const uint4 v = load_shared16(x + n * 8 * U::kStride + 256 * (from + i));
-            mma_bf16(acc[n], ga.x, ua.x, ga.y, ua.y, v.x, v.y);
-            mma_bf16(acc[n], ga.z, ua.z, ga.w, ua.w, v.z, v.w);
-          }
-        }
+      for (int i = 0; i < kFewUpAhead; ++i) {
+        if (from + i >= steps) break;
+        mma_bf16(acc, a[i].x, b[i].x, a[i].y, b[i].y, v[i].x, v[i].y);
+        mma_bf16(acc, a[i].z, b[i].z, a[i].w, b[i].w, v[i].z, v[i].w);
+        if (from + i + kFewUpAhead < steps) fetch(i, from + i + kFewUpAhead);
       }
     }
-    __syncthreads();
-    float* sums = reinterpret_cast<float*>(up_shared);  // [tile of channels][split][token tile][4][lane]
 #pragma unroll
-    for (int n = 0; n < TILES; ++n)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) sums[((warp * TILES + n) * 4 + i) * 32 + lane] = acc[n][i];
+    for (int i = 0; i < 4; ++i) sums[warp][i][lane] = acc[i];
     __syncthreads();
-    for (int i = tid; i < kUpChannels * 8 * TILES; i += kThreads) {
-      const int c = i % kUpChannels, token = i / kUpChannels;
-      if (token >= tokens) continue;
-      const int from_lane = (c & 7) * 4 + ((token & 7) >> 1);
+    if (tid < 64 && pass + tid / 8 < count) {
+      const int channel = tid & 7, token = tid >> 3, from = 4 * channel + (token >> 1);
       float gu[2];
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
-        const float* of = sums + ((c / 8 * kSplits * TILES + token / 8) * 4 + 2 * half + (token & 1)) * 32 + from_lane;
-        float sum = of[0];
-#pragma unroll
-        for (int j = 1; j < kSplits; ++j) sum += of[j * TILES * 128];
-        gu[half] = sum;
+        const int i = 2 * half + (token & 1);
+        gu[half] = (sums[0][i][from] + sums[1][i][from]) + (sums[2][i][from] + sums[3][i][from]);
       }
-      store_activation(s, static_cast<size_t>(s.pairs[first + pass + token]) * L.I + c0 + c,
+      store_activation(s, static_cast<size_t>(pair_at(few.mask, pass + token)) * L.I + c0 + channel,
                        gated(gu[0], gu[1], L.activation));
     }
     __syncthreads();
   }
 }
 
-// ---- down ------------------------------------------------------------------------------------------
-constexpr int kDownColumns = 128;  // of a CTA: two warps' 64
-constexpr int kDownAhead = 2;      // steps of 16 channels whose rows are on their way
+constexpr int kFewDownThreads = 256;
+constexpr int kFewDownWarps = kFewDownThreads / 32;
+constexpr int kFewDownColumns = 64;  // of a cluster
+constexpr int kFewDownAhead = 3;     // steps of 16 channels whose rows are on their way
+constexpr int kFewRanks = 8;         // CTAs of a cluster
 
-// grid (H / 128, experts that can have pairs).  A thread has 16 bytes, eight outputs, of four channels' rows; the
-// first operand's registers pair two channels of one output, which two byte permutations per pair of words do.
-template <int TILES>
-__global__ void __launch_bounds__(kThreads, 2) k_experts_down(Experts L, Scratch s) {
-  extern __shared__ __align__(16) uint8_t down_shared[];
-  grid_dependency_wait();
-  grid_dependency_release();
-  if (static_cast<int>(blockIdx.y) >= s.counts[0]) return;
-  constexpr int kTokens = 8 * TILES;
+// grid (8 H / 64): a cluster has 64 outputs of all tokens, its CTAs share the experts, or where those are few
+// their channels; a CTA's warps share a CTA's channels.  A thread has 16 bytes, eight outputs, of four channels'
+// rows; the first operand's registers pair two channels of one output, which two byte permutations per pair of
+// words do.  The first rows are on their way before the kernel before this one has ended.
+// Sums of warps and of CTAs are added in their order.
+__global__ void __launch_bounds__(kFewDownThreads, 2)
+    k_few_down(Experts L, Scratch s, Routes routes, __nv_bfloat16* out) {
+  __shared__ float parts[kFewDownWarps][8][kFewDownColumns];
+  __shared__ float total[kFewPairs][kFewDownColumns];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
-  const int split = warp & (kSplits - 1), half = warp / kSplits;
-  const int e = s.busy[blockIdx.y], first = s.offsets[e], pairs = s.offsets[e + 1] - first;
-  const int h0 = blockIdx.x * kDownColumns + 64 * half;
-  const int all = L.I / 16, begin = all * split / kSplits, end = all * (split + 1) / kSplits;
-  const int stride = (2 * L.I + 127) / 128 * 128 + 32;  // bytes of a row of activations
-  const __nv_bfloat16* rows = L.down + (static_cast<size_t>(e) * L.I + 4 * t) * L.H + h0 + 8 * g;
-  auto fetch = [&](uint4 (&w)[4], int step) {
+  const int rank = blockIdx.x % kFewRanks, h0 = blockIdx.x / kFewRanks * kFewDownColumns;
+  for (int i = tid; i < routes.tokens * kFewDownColumns; i += kFewDownThreads) total[0][i] = 0.0f;
+  const Few all = few_pairs(routes, L.K, L.E, 0);
+  const int splits = all.experts >= 5 ? 1 : all.experts >= 3 ? 2 : all.experts == 2 ? 4 : 8;
+  bool waited = false;
+  for (int unit = rank; unit < all.experts * splits; unit += kFewRanks) {
+    const Few few = few_pairs(routes, L.K, L.E, unit / splits);
+    const int count = __popc(few.mask), part = unit % splits * kFewDownWarps + warp, pieces = splits * kFewDownWarps;
+    const int begin = L.I / 16 * part / pieces, end = L.I / 16 * (part + 1) / pieces;
+    const __nv_bfloat16* rows = L.down + (static_cast<size_t>(few.e) * L.I + 4 * t) * L.H + h0 + 8 * g;
+    for (int pass = 0; pass < count; pass += 8) {
+      uint4 w[kFewDownAhead][4];
+      auto fetch = [&](int i, int step) {
 #pragma unroll
-    for (int r = 0; r < 4; ++r) w[r] = load_stream16(rows + static_cast<size_t>(16 * step + r) * L.H);
-  };
-
-  for (int pass = 0; pass < pairs; pass += kTokens) {
-    const int tokens = min(kTokens, pairs - pass);
-    uint4 w[kDownAhead][4];
+        for (int r = 0; r < 4; ++r) w[i][r] = load_stream16(rows + static_cast<size_t>(16 * step + r) * L.H);
+      };
 #pragma unroll
-    for (int i = 0; i < kDownAhead; ++i)
-      if (begin + i < end) fetch(w[i], begin + i);
-    __syncthreads();
-    for (int i = tid; i < tokens * (L.I / 8); i += kThreads) {
-      const int row = i / (L.I / 8), piece = i - row * (L.I / 8);
-      const size_t from = static_cast<size_t>(s.pairs[first + pass + row]) * L.I + 8 * piece;
-      copy_async16(shared_u32(down_shared + row * stride + 16 * piece), s.activations + from);
-      copy_async16(shared_u32(down_shared + (kTokens + row) * stride + 16 * piece), s.rests + from);
-    }
-    copy_async_commit();
-    copy_async_wait<0>();
-    __syncthreads();
-    float acc[TILES][4][4] = {};
-    const uint32_t x = shared_u32(down_shared) + g * stride + 8 * t;
-    for (int from = begin; from < end; from += kDownAhead) {
+      for (int i = 0; i < kFewDownAhead; ++i)
+        if (begin + i < end) fetch(i, begin + i);
+      if (!waited) grid_dependency_wait();
+      waited = true;
+      const int pair = pair_at(few.mask, pass + g);
+      const size_t at = static_cast<size_t>(max(pair, 0)) * L.I + 4 * t;
+      float acc[4][4] = {};
+      for (int from = begin; from < end; from += kFewDownAhead) {
 #pragma unroll
-      for (int i = 0; i < kDownAhead; ++i) {
-        const int step = from + i;
-        if (step >= end) break;
-        uint32_t a[4][4];
-        const uint32_t* v[4] = {&w[i][0].x, &w[i][1].x, &w[i][2].x, &w[i][3].x};
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          a[j][0] = __byte_perm(v[0][j], v[1][j], 0x5410);
-          a[j][1] = __byte_perm(v[0][j], v[1][j], 0x7632);
-          a[j][2] = __byte_perm(v[2][j], v[3][j], 0x5410);
-          a[j][3] = __byte_perm(v[2][j], v[3][j], 0x7632);
-        }
-        if (step + kDownAhead < end) fetch(w[i], step + kDownAhead);
-#pragma unroll
-        for (int n = 0; n < TILES; ++n) {
-#pragma unroll
-          for (int term = 0; term < 2; ++term) {
-            uint32_t b0, b1;
-            asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];"
-                         : "=r"(b0), "=r"(b1)
-                         : "r"(x + (term * kTokens + n * 8) * stride + 32 * step));
-#pragma unroll
-            for (int j = 0; j < 4; ++j) mma_bf16(acc[n][j], a[j][0], a[j][1], a[j][2], a[j][3], b0, b1);
+        for (int i = 0; i < kFewDownAhead; ++i) {
+          const int step = from + i;
+          if (step >= end) break;
+          uint2 b[2] = {};
+          if (pair >= 0) {
+            b[0] = *reinterpret_cast<const uint2*>(s.activations + at + 16 * step);
+            b[1] = *reinterpret_cast<const uint2*>(s.rests + at + 16 * step);
           }
+          const uint32_t* v[4] = {&w[i][0].x, &w[i][1].x, &w[i][2].x, &w[i][3].x};
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const uint32_t a0 = __byte_perm(v[0][j], v[1][j], 0x5410), a1 = __byte_perm(v[0][j], v[1][j], 0x7632);
+            const uint32_t a2 = __byte_perm(v[2][j], v[3][j], 0x5410), a3 = __byte_perm(v[2][j], v[3][j], 0x7632);
+            mma_bf16(acc[j], a0, a1, a2, a3, b[0].x, b[0].y);
+            mma_bf16(acc[j], a0, a1, a2, a3, b[1].x, b[1].y);
+          }
+          if (step + kFewDownAhead < end) fetch(i, step + kFewDownAhead);
         }
       }
-    }
-    __syncthreads();
-    float* sums = reinterpret_cast<float*>(down_shared);  // [half][split][token][64]
-#pragma unroll
-    for (int n = 0; n < TILES; ++n)
+      __syncthreads();  // the parts before have been added
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
-        float4* to = reinterpret_cast<float4*>(sums + (static_cast<size_t>(warp) * kTokens + 8 * n + 2 * t + c) * 64 + 8 * g);
-        to[0] = make_float4(acc[n][0][c], acc[n][0][2 + c], acc[n][1][c], acc[n][1][2 + c]);
-        to[1] = make_float4(acc[n][2][c], acc[n][2][2 + c], acc[n][3][c], acc[n][3][2 + c]);
+        float4* to = reinterpret_cast<float4*>(&parts[warp][2 * t + c][8 * g]);
+        to[0] = make_float4(acc[0][c], acc[0][2 + c], acc[1][c], acc[1][2 + c]);
+        to[1] = make_float4(acc[2][c], acc[2][2 + c], acc[3][c], acc[3][2 + c]);
       }
-    __syncthreads();
-    for (int i = tid; i < tokens * (kDownColumns / 4); i += kThreads) {
-      const int token = i / (kDownColumns / 4), column = i % (kDownColumns / 4) * 4;
-      const float* of = sums + (static_cast<size_t>(column / 64 * kSplits) * kTokens + token) * 64 + column % 64;
-      float4 sum = *reinterpret_cast<const float4*>(of);
+      __syncthreads();
+      // A token that has this expert twice: its pairs are added one after another.
+      const int tokens = min(8, count - pass), together = few.twice ? 1 : tokens;
+      for (int from = 0; from < tokens; from += together) {
+        for (int i = tid; i < together * kFewDownColumns; i += kFewDownThreads) {
+          const int token = from + i / kFewDownColumns, column = i % kFewDownColumns;
+          float sum = parts[0][token][column];
 #pragma unroll
-      for (int j = 1; j < kSplits; ++j) {
-        const float4 more = *reinterpret_cast<const float4*>(of + static_cast<size_t>(j) * kTokens * 64);
-        sum = make_float4(sum.x + more.x, sum.y + more.y, sum.z + more.z, sum.w + more.w);
+          for (int j = 1; j < kFewDownWarps; ++j) sum += parts[j][token][column];
+          const int of = pair_at(few.mask, pass + token);
+          float& to = total[of / L.K][column];
+          to = __fmaf_rn(routes.weight(of), sum, to);
+        }
+        if (few.twice) __syncthreads();
       }
-      const int pair = s.pairs[first + pass + token];
-      *reinterpret_cast<float4*>(s.sums + static_cast<size_t>(pair) * L.H + blockIdx.x * kDownColumns + column) = sum;
     }
-    __syncthreads();
   }
-}
-
-template <int TILES>
-static size_t down_shared_bytes(int I) {
-  const size_t rows = 2 * 8 * TILES * static_cast<size_t>((2 * I + 127) / 128 * 128 + 32);
-  return std::max(rows, static_cast<size_t>(kThreads / 32) * 8 * TILES * 64 * sizeof(float));
+  if (!waited) grid_dependency_wait();
+  grid_dependency_release();
+  __syncthreads();
+  cluster_meet();
+  constexpr int kShare = kFewDownColumns / kFewRanks;
+  for (int i = tid; i < routes.tokens * kShare; i += kFewDownThreads) {
+    const int token = i / kShare, column = rank * kShare + i % kShare;
+    float sum = 0.0f;
+#pragma unroll
+    for (int j = 0; j < kFewRanks; ++j) sum += *of_rank(&total[token][column], j);
+    out[static_cast<size_t>(token) * L.H + h0 + column] = __float2bfloat16_rn(sum);
+  }
+  cluster_meet();  // the others' shared memory has been read
 }
 
 #include "cfm_experts_tc.cuh"
@@ -435,7 +407,7 @@ int64_t align256(int64_t v) { return (v + 255) / 256 * 256; }
 int check_experts(const cfm_experts* x) {
   if (!x) return CFM_E_NULL;
   if (x->hidden < 128 || x->hidden % 128 || x->width < 16 || x->width % 16 || x->experts < 1 ||
-      x->experts > kMaxExperts || x->top_k < 1 || x->top_k > 32 || x->hidden > 65536 || x->width > kMaxWidth)
+      x->experts > kMaxExperts || x->top_k < 1 || x->top_k > 32 || x->hidden > 65536 || x->width > 65536)
     return CFM_E_SHAPE;
   if (x->activation != CFM_ACT_SILU && x->activation != CFM_ACT_GELU_TANH) return CFM_E_UNSUPPORTED;
   return 0;
@@ -453,10 +425,8 @@ int64_t lay_out(const cfm_experts* x, int64_t capacity, void* base, Scratch* s) 
   Scratch* to = s ? s : &none;
   const int64_t pairs = capacity * x->top_k;
   take(&to->status, 4);
-  take(&to->offsets, x->experts + 1);
   take(&to->pairs, pairs);
   take(&to->tokens, pairs);
-  take(&to->busy, x->experts);
   take(&to->passes, std::min<int64_t>(x->experts, pairs) + pairs / kLeastPass);
   take(&to->counts, 4);
   take(&to->activations, pairs * x->width);
@@ -471,15 +441,12 @@ int allow_shared(K kernel, size_t bytes) {
   return static_cast<int>(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(bytes)));
 }
 
-template <int TILES>
-int run_tiles(const Experts& L, const Scratch& s, const __nv_bfloat16* hidden, int busy, cudaStream_t stream) {
-  const size_t down = down_shared_bytes<TILES>(L.I);
-  int code = allow_shared(k_experts_up<TILES>, Up<TILES>::kBytes);
-  if (!code) code = allow_shared(k_experts_down<TILES>, down);
-  if (code) return code;
-  launch_dependent(k_experts_up<TILES>, dim3(L.I / kUpChannels, busy), dim3(kThreads), Up<TILES>::kBytes, stream, L, s, hidden);
-  launch_dependent(k_experts_down<TILES>, dim3(L.H / kDownColumns, busy), dim3(kThreads), down, stream, L, s);
-  return 0;
+int run_few(const Experts& L, const Scratch& s, const Routes& routes, const __nv_bfloat16* hidden, int busy,
+            __nv_bfloat16* out, cudaStream_t stream) {
+  launch_dependent(k_few_up, dim3(L.I / 8, busy), dim3(kFewUpThreads), 0, stream, L, s, routes, hidden);
+  launch_clusters(k_few_down, dim3(L.H / kFewDownColumns * kFewRanks), dim3(kFewDownThreads), 0, kFewRanks, stream, L, s,
+                  routes, out);
+  return launched();
 }
 
 // The map of a matrix [rows, columns] in boxes of 64 columns and 64 rows, swizzled by 128 bytes.
@@ -558,16 +525,17 @@ int cfm_experts_forward(const cfm_experts* layer, void* workspace, int32_t capac
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
   const int64_t pairs = static_cast<int64_t>(L.K) * call->tokens;
   const int busy = static_cast<int>(std::min<int64_t>(L.E, pairs));
+  auto* out = static_cast<__nv_bfloat16*>(call->out);
+  if (pairs <= kFewPairs) return run_few(L, s, routes, hidden, busy, out, st);
   const int pass = pass_pairs(pairs, busy);
   launch_dependent(k_group_pairs, dim3(1), dim3(kGroupThreads), sizeof(int) * L.E, st, routes, L.E, L.K, pass, s);
-  const int code = pairs <= 32    ? run_tiles<1>(L, s, hidden, busy, st)
-                   : pass == 32   ? run_tensor<32>(L, s, hidden, pairs, st)
-                   : pass == 64   ? run_tensor<64>(L, s, hidden, pairs, st)
-                   : pass == 128  ? run_tensor<128>(L, s, hidden, pairs, st)
-                                  : run_tensor<192>(L, s, hidden, pairs, st);
+  const int code = pass == 32    ? run_tensor<32>(L, s, hidden, pairs, st)
+                   : pass == 64  ? run_tensor<64>(L, s, hidden, pairs, st)
+                   : pass == 128 ? run_tensor<128>(L, s, hidden, pairs, st)
+                                 : run_tensor<192>(L, s, hidden, pairs, st);
   if (code) return code;
   launch_dependent(k_experts_mix, dim3(call->tokens, (L.H + 8 * kMixThreads - 1) / (8 * kMixThreads)), dim3(kMixThreads), 0,
-                   st, L, s, routes, static_cast<__nv_bfloat16*>(call->out));
+                   st, L, s, routes, out);
   return launched();
 }
 

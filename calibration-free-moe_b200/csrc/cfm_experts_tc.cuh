@@ -152,7 +152,7 @@ __global__ void __launch_bounds__(Tensor<TOKENS, DOWN>::kThreads, 1)
   const int I = L.I, H = L.H;
   const int tiles = DOWN ? H / kTensorRows : (I + kUpTile - 1) / kUpTile;
   const int chunks = DOWN ? (I + kTensorColumns - 1) / kTensorColumns : H / kTensorColumns;
-  const int items = __ldcg(&s.counts[1]) * tiles;
+  const int items = __ldcg(&s.counts[0]) * tiles;
   // Expert, first pair, pairs.  Each role asks for an item's pass while it is at the item before.
   auto pass_of = [&](int item) { return item < items ? __ldcg(&s.passes[item / tiles]) : make_int4(0, 0, 0, 0); };
   const int step = gridDim.x;

@@ -212,28 +212,6 @@ struct Best {
   }
 };
 
-// ---- clusters --------------------------------------------------------------------------------------
-__device__ __forceinline__ int cluster_rank() {
-  uint32_t r;
-  asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
-  return static_cast<int>(r);
-}
-__device__ __forceinline__ int cluster_size() {
-  uint32_t r;
-  asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(r));
-  return static_cast<int>(r);
-}
-__device__ __forceinline__ void cluster_meet() {
-  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
-// What lies at this place of another CTA's shared memory.
-template <typename V>
-__device__ __forceinline__ const V* of_rank(const V* mine, int rank) {
-  V* other;
-  asm("mapa.u64 %0, %1, %2;" : "=l"(other) : "l"(mine), "r"(rank));
-  return other;
-}
-
 // ---- router ----------------------------------------------------------------------------------------
 constexpr int kRouteRows = 4;       // a warp each
 constexpr int kRouteColumns = 1024;

@@ -41,7 +41,7 @@ class RoutedExperts:
 
     gate_up BF16 `[E, 2I, H]` (gate rows, then up rows), contiguous; down BF16, logical `[E, H, I]`
     in the storage of `channel_major_down`: what `ProgressiveReader` takes, and the two may share
-    them.  H a multiple of 128, I of 16 up to 4096, E up to 4096, top_k up to 32.  Calls take up to
+    them.  H a multiple of 128, I of 16, E up to 4096, top_k up to 32.  Calls take up to
     `max_tokens` tokens.  Inference only.
     """
 

@@ -454,7 +454,7 @@ int cfm_compare_logits(const cfm_rows* reference, const cfm_rows* logits, float*
 /* The routed experts of a layer as a whole: dimensions and weights, as in cfm_layer. */
 typedef struct cfm_experts {
   int32_t hidden;         /* H, multiple of 128, at most 65536                 */
-  int32_t width;          /* I, multiple of 16, at most 4096                   */
+  int32_t width;          /* I, multiple of 16, at most 65536                  */
   int32_t experts;        /* E <= 4096                                         */
   int32_t top_k;          /* K <= 32                                           */
   int32_t activation;     /* CFM_ACT_*                                         */

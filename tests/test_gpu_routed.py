@@ -118,12 +118,24 @@ def test_all_rows_padding_or_without_an_expert():
     assert not run(x, torch.full_like(ids, -1), weights).any()
 
 
-def test_the_same_expert_twice_and_one_expert_for_all():
+@pytest.mark.parametrize("tokens", [1, 5, 10, 50])
+def test_the_same_expert_twice_and_one_expert_for_all(tokens):
     gate_up, down = layer(256, 48, 3)
-    x, ids, weights = batch(50, 256, 3, 3)
-    check(gate_up, down, x, torch.ones_like(ids), weights)
+    x, ids, weights = batch(tokens, 256, 3, 3)
+    run = RoutedExperts(gate_up, down, 3, tokens)
+    got = check(gate_up, down, x, torch.ones_like(ids), weights, run=run)
+    assert torch.equal(run(x, torch.ones_like(ids), weights), got)
     ids[:, 2] = ids[:, 0]
+    check(gate_up, down, x, ids, weights, run=run)
+
+
+@pytest.mark.parametrize("tokens,top_k", [(32, 1), (16, 2), (1, 32), (3, 10), (4, 8), (33, 1), (11, 3)])
+def test_few_pairs_and_one_more(tokens, top_k):
+    gate_up, down = layer(384, 80, 40)
+    x, ids, weights = batch(tokens, 384, 40, top_k)
     check(gate_up, down, x, ids, weights)
+    check(gate_up, down, x, ids % 3, weights)  # many pairs per expert, most tokens with an expert twice
+    check(gate_up, down, x, ids % 9, weights)
 
 
 def test_a_tokens_output_does_not_depend_on_the_batch():
