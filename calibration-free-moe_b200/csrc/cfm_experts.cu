@@ -179,69 +179,106 @@ __global__ void __launch_bounds__(kGroupThreads) k_group_pairs(Routes routes, in
 }
 
 // ---- few pairs -------------------------------------------------------------------------------------
-// Calls of up to 32 pairs in two launches.  The weights go from global memory straight into the registers of
+// Calls of up to 16 pairs in two launches (two tokens of the 128-expert layer 36 us, 43 on the tensor-core path; three 50
+// and 50, four 65 and 62).  The weights go from global memory straight into the registers of
 // warp-level tensor-core products (m16n8k16), whose eight columns are the tokens of an expert.  Every warp
 // groups the pairs by itself, a pair per lane.
-constexpr int kFewPairs = 32;
+constexpr int kFewPairs = 16;
 
 struct Few {
   int e;          // expert, -1: there are fewer
   unsigned mask;  // its pairs
-  int experts;    // number of busy ones
   bool twice;     // some token has it twice
 };
-// The `which`-th busy expert, in the order of first pairs.
-__device__ __forceinline__ Few few_pairs(const Routes& routes, int K, int E, int which) {
-  const int lane = threadIdx.x & 31;
-  const int e = lane < routes.tokens * K ? routes.expert(lane, K, E) : -1;
-  const unsigned same = __match_any_sync(kFull, e);
-  unsigned first = __ballot_sync(kFull, e >= 0 && lane == __ffs(same) - 1);
-  Few few = {-1, 0, __popc(first), false};
-  if (which >= few.experts) return few;
-  for (int i = 0; i < which; ++i) first &= first - 1;
-  const int from = __ffs(first) - 1;
-  few.e = __shfl_sync(kFull, e, from);
-  few.mask = __shfl_sync(kFull, same, from);
-  const unsigned token = __match_any_sync(kFull, lane / K);
-  few.twice = __any_sync(kFull, e == few.e && (token & few.mask & ~(1u << lane)) != 0);
-  return few;
-}
+// Of a warp, a pair per lane.
+struct FewGroups {
+  int e;           // the lane's expert
+  unsigned same;   // lanes with that expert
+  unsigned first;  // the first lane of every busy expert
+  unsigned again;  // lanes of the same token with that expert
+
+  __device__ FewGroups(const Routes& routes, int K, int E) {
+    const int lane = threadIdx.x & 31;
+    e = lane < routes.tokens * K ? routes.expert(lane, K, E) : -1;
+    same = __match_any_sync(kFull, e);
+    first = __ballot_sync(kFull, e >= 0 && lane == __ffs(same) - 1);
+    again = same & __match_any_sync(kFull, lane / K) & ~(1u << lane);
+  }
+  __device__ int experts() const { return __popc(first); }
+  // The `which`-th busy expert, in the order of first pairs.
+  __device__ Few group(int which) const {
+    if (which >= experts()) return {-1, 0, false};
+    unsigned rest = first;
+    for (int i = 0; i < which; ++i) rest &= rest - 1;
+    const int from = __ffs(rest) - 1;
+    Few few;
+    few.e = __shfl_sync(kFull, e, from);
+    few.mask = __shfl_sync(kFull, same, from);
+    few.twice = __any_sync(kFull, e == few.e && again);
+    return few;
+  }
+};
 // The pair at a place among the set bits, -1 behind them.
 __device__ __forceinline__ int pair_at(unsigned mask, int place) {
   for (int i = 0; i < place; ++i) mask &= mask - 1;
   return __ffs(mask) - 1;
 }
 
-constexpr int kFewUpThreads = 128;
-constexpr int kFewUpAhead = 4;  // steps of 32 columns whose rows are on their way
+__device__ __forceinline__ void prefetch_row(const void* row, int bytes) {
+  asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(row), "r"(bytes) : "memory");
+}
 
-// grid (I / 8, experts that can have pairs).  A CTA has eight channels, its warps share the columns.  A thread
-// has 16 bytes of a gate row and of an up row, whose elements are the k of two instructions, and the same
-// of a token's row; gate and up of a channel end in one thread.
-__global__ void __launch_bounds__(kFewUpThreads, 6)
+constexpr int kFewUpThreads = 128;
+constexpr int kFewUpWarps = kFewUpThreads / 32;
+constexpr int kFewUpAhead = 4;  // steps of 32 columns whose rows are on their way
+constexpr int kFewUpPerSm = 6;
+constexpr int kFewUpBlock = 64;  // columns
+
+// Items are eight channels of an expert; a CTA's warps share the columns, and it asks for its next item's first
+// rows before it adds up the sums of the last.  A thread has 16 bytes of a gate row and of an up row, whose elements
+// are the k of two instructions, and the same of a token's row; gate and up of a channel end in one thread.
+__global__ void __launch_bounds__(kFewUpThreads, kFewUpPerSm)
     k_few_up(Experts L, Scratch s, Routes routes, const __nv_bfloat16* hidden) {
-  __shared__ float sums[kFewUpThreads / 32][4][32];
+  __shared__ float sums[kFewUpWarps][4][32];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
   grid_dependency_wait();
   grid_dependency_release();
-  const Few few = few_pairs(routes, L.K, L.E, blockIdx.y);
-  if (few.e < 0) return;
-  const int count = __popc(few.mask), c0 = 8 * blockIdx.x, steps = L.H / 128, at = 32 * warp + 8 * t;
-  const __nv_bfloat16* gate = L.gate_up + (static_cast<size_t>(few.e) * 2 * L.I + c0 + g) * L.H + at;
-  const __nv_bfloat16* up = gate + static_cast<size_t>(L.I) * L.H;
-  for (int pass = 0; pass < count; pass += 8) {
-    const int pair = pair_at(few.mask, pass + g);
-    const __nv_bfloat16* x = hidden + static_cast<size_t>(max(pair, 0) / L.K) * L.H + at;
-    float acc[4] = {};
-    uint4 a[kFewUpAhead], b[kFewUpAhead], v[kFewUpAhead];
-    auto fetch = [&](int i, int step) {
-      a[i] = load_stream16(gate + 128 * step);
-      b[i] = load_stream16(up + 128 * step);
-      v[i] = pair >= 0 ? __ldg(reinterpret_cast<const uint4*>(x + 128 * step)) : make_uint4(0, 0, 0, 0);
-    };
+  // A warp's columns are every fourth block of kFewUpBlock.
+  constexpr int kPer = kFewUpBlock / 32;
+  const int steps = (L.H / kFewUpBlock - warp + kFewUpWarps - 1) / kFewUpWarps * kPer, at = kFewUpBlock * warp + 8 * t, tiles = L.I / 8;
+  auto column = [](int step) { return step / kPer * (kFewUpWarps * kFewUpBlock) + step % kPer * 32; };
+  const FewGroups groups(routes, L.K, L.E);
+  Few few;
+  int count, c0, pass, pair;
+  const __nv_bfloat16 *gate, *up, *x;
+  uint4 a[kFewUpAhead], b[kFewUpAhead], v[kFewUpAhead];
+  auto fetch = [&](int i, int step) {
+    a[i] = load_stream16(gate + column(step));
+    b[i] = load_stream16(up + column(step));
+    v[i] = pair >= 0 ? __ldg(reinterpret_cast<const uint4*>(x + column(step))) : make_uint4(0, 0, 0, 0);
+  };
+  // The first rows of a pass over an item.
+  auto start = [&](int from) {
+    pass = from;
+    pair = pair_at(few.mask, pass + g);
+    x = hidden + static_cast<size_t>(max(pair, 0) / L.K) * L.H + at;
 #pragma unroll
     for (int i = 0; i < kFewUpAhead; ++i)
       if (i < steps) fetch(i, i);
+  };
+  auto open = [&](int item) {
+    few = groups.group(item / tiles);
+    if (few.e < 0) return;
+    count = __popc(few.mask);
+    c0 = item % tiles * 8;
+    gate = L.gate_up + (static_cast<size_t>(few.e) * 2 * L.I + c0 + g) * L.H + at;
+    up = gate + static_cast<size_t>(L.I) * L.H;
+    start(0);
+  };
+  int item = blockIdx.x;
+  open(item);
+  while (few.e >= 0) {
+    float acc[4] = {};
     for (int from = 0; from < steps; from += kFewUpAhead) {
 #pragma unroll
       for (int i = 0; i < kFewUpAhead; ++i) {
@@ -251,18 +288,32 @@ __global__ void __launch_bounds__(kFewUpThreads, 6)
         if (from + i + kFewUpAhead < steps) fetch(i, from + i + kFewUpAhead);
       }
     }
+    const unsigned mask = few.mask;
+    const int tokens = min(8, count - pass), first = pass, channels = c0;
+    // The down rows of these channels, one after another in memory, come to L2 while the sums are added up and the
+    // next kernel starts.
+    if (tid < 8 && pass == 0) prefetch_row(L.down + (static_cast<size_t>(few.e) * L.I + c0 + tid) * L.H, 2 * L.H);
+    if (pass + 8 < count) {
+      start(pass + 8);
+    } else {
+      item += gridDim.x;
+      open(item);
+    }
 #pragma unroll
     for (int i = 0; i < 4; ++i) sums[warp][i][lane] = acc[i];
     __syncthreads();
-    if (tid < 64 && pass + tid / 8 < count) {
+    if (tid < 8 * tokens) {
       const int channel = tid & 7, token = tid >> 3, from = 4 * channel + (token >> 1);
       float gu[2];
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
         const int i = 2 * half + (token & 1);
-        gu[half] = (sums[0][i][from] + sums[1][i][from]) + (sums[2][i][from] + sums[3][i][from]);
+        float sum = sums[0][i][from];
+#pragma unroll
+        for (int j = 1; j < kFewUpWarps; ++j) sum += sums[j][i][from];
+        gu[half] = sum;
       }
-      store_activation(s, static_cast<size_t>(pair_at(few.mask, pass + token)) * L.I + c0 + channel,
+      store_activation(s, static_cast<size_t>(pair_at(mask, first + token)) * L.I + channels + channel,
                        gated(gu[0], gu[1], L.activation));
     }
     __syncthreads();
@@ -272,7 +323,7 @@ __global__ void __launch_bounds__(kFewUpThreads, 6)
 constexpr int kFewDownThreads = 256;
 constexpr int kFewDownWarps = kFewDownThreads / 32;
 constexpr int kFewDownColumns = 64;  // of a cluster
-constexpr int kFewDownAhead = 3;     // steps of 16 channels whose rows are on their way
+constexpr int kFewDownAhead = 4;     // steps of 16 channels whose rows are on their way
 constexpr int kFewRanks = 8;         // CTAs of a cluster
 
 // grid (8 H / 64): a cluster has 64 outputs of all tokens, its CTAs share the experts, or where those are few
@@ -287,11 +338,11 @@ __global__ void __launch_bounds__(kFewDownThreads, 2)
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
   const int rank = blockIdx.x % kFewRanks, h0 = blockIdx.x / kFewRanks * kFewDownColumns;
   for (int i = tid; i < routes.tokens * kFewDownColumns; i += kFewDownThreads) total[0][i] = 0.0f;
-  const Few all = few_pairs(routes, L.K, L.E, 0);
-  const int splits = all.experts >= 5 ? 1 : all.experts >= 3 ? 2 : all.experts == 2 ? 4 : 8;
+  const FewGroups groups(routes, L.K, L.E);
+  const int experts = groups.experts(), splits = experts >= 5 ? 1 : experts >= 3 ? 2 : experts == 2 ? 4 : 8;
   bool waited = false;
-  for (int unit = rank; unit < all.experts * splits; unit += kFewRanks) {
-    const Few few = few_pairs(routes, L.K, L.E, unit / splits);
+  for (int unit = rank; unit < experts * splits; unit += kFewRanks) {
+    const Few few = groups.group(unit / splits);
     const int count = __popc(few.mask), part = unit % splits * kFewDownWarps + warp, pieces = splits * kFewDownWarps;
     const int begin = L.I / 16 * part / pieces, end = L.I / 16 * (part + 1) / pieces;
     const __nv_bfloat16* rows = L.down + (static_cast<size_t>(few.e) * L.I + 4 * t) * L.H + h0 + 8 * g;
@@ -310,15 +361,18 @@ __global__ void __launch_bounds__(kFewDownThreads, 2)
       const size_t at = static_cast<size_t>(max(pair, 0)) * L.I + 4 * t;
       float acc[4][4] = {};
       for (int from = begin; from < end; from += kFewDownAhead) {
+        uint2 x[kFewDownAhead][2];
+#pragma unroll
+        for (int i = 0; i < kFewDownAhead; ++i) {
+          const bool has = pair >= 0 && from + i < end;
+          x[i][0] = has ? *reinterpret_cast<const uint2*>(s.activations + at + 16 * (from + i)) : make_uint2(0, 0);
+          x[i][1] = has ? *reinterpret_cast<const uint2*>(s.rests + at + 16 * (from + i)) : make_uint2(0, 0);
+        }
 #pragma unroll
         for (int i = 0; i < kFewDownAhead; ++i) {
           const int step = from + i;
           if (step >= end) break;
-          uint2 b[2] = {};
-          if (pair >= 0) {
-            b[0] = *reinterpret_cast<const uint2*>(s.activations + at + 16 * step);
-            b[1] = *reinterpret_cast<const uint2*>(s.rests + at + 16 * step);
-          }
+          const uint2* b = x[i];
           const uint32_t* v[4] = {&w[i][0].x, &w[i][1].x, &w[i][2].x, &w[i][3].x};
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
@@ -443,7 +497,8 @@ int allow_shared(K kernel, size_t bytes) {
 
 int run_few(const Experts& L, const Scratch& s, const Routes& routes, const __nv_bfloat16* hidden, int busy,
             __nv_bfloat16* out, cudaStream_t stream) {
-  launch_dependent(k_few_up, dim3(L.I / 8, busy), dim3(kFewUpThreads), 0, stream, L, s, routes, hidden);
+  const int64_t items = static_cast<int64_t>(busy) * (L.I / 8);
+  launch_dependent(k_few_up, dim3(static_cast<unsigned>(std::min<int64_t>(items, 148 * kFewUpPerSm))), dim3(kFewUpThreads), 0, stream, L, s, routes, hidden);
   launch_clusters(k_few_down, dim3(L.H / kFewDownColumns * kFewRanks), dim3(kFewDownThreads), 0, kFewRanks, stream, L, s,
                   routes, out);
   return launched();

@@ -474,7 +474,7 @@ int64_t cfm_experts_workspace_bytes(const cfm_experts* layer, int32_t capacity);
  * cfm_reader_forward takes them; hidden, out and the weights on 16-byte boundaries.  An id outside of [0, E) adds nothing; a token may have an expert
  * more than once.  Padding rows read nothing and produce zero rows.  Sums are FP32, activations keep
  * 16 bits, the output is rounded once.  A token's bits do not depend on the other tokens, except
- * between calls of up to 32 (token, slot) pairs and larger ones. */
+ * between calls of up to 16 (token, slot) pairs and larger ones. */
 int cfm_experts_forward(const cfm_experts* layer, void* workspace, int32_t capacity,
                         const cfm_call* call, void* stream);
 

@@ -129,7 +129,7 @@ def test_the_same_expert_twice_and_one_expert_for_all(tokens):
     check(gate_up, down, x, ids, weights, run=run)
 
 
-@pytest.mark.parametrize("tokens,top_k", [(32, 1), (16, 2), (1, 32), (3, 10), (4, 8), (33, 1), (11, 3)])
+@pytest.mark.parametrize("tokens,top_k", [(16, 1), (8, 2), (1, 16), (2, 8), (1, 9), (17, 1), (6, 3), (1, 32), (32, 1)])
 def test_few_pairs_and_one_more(tokens, top_k):
     gate_up, down = layer(384, 80, 40)
     x, ids, weights = batch(tokens, 384, 40, top_k)
@@ -139,11 +139,11 @@ def test_few_pairs_and_one_more(tokens, top_k):
 
 
 def test_a_tokens_output_does_not_depend_on_the_batch():
-    """Among calls of up to 32 pairs, and among larger ones."""
+    """Among calls of up to 16 pairs, and among larger ones."""
     gate_up, down = layer(1152, 96, 4)
     x, ids, weights = batch(300, 1152, 4, 2)
     run = RoutedExperts(gate_up, down, 2, 300)
-    for whole, parts in ((slice(0, 16), (slice(0, 1), slice(3, 12))),
+    for whole, parts in ((slice(0, 8), (slice(0, 1), slice(2, 7))),
                          (slice(0, 300), (slice(3, 20), slice(20, 52), slice(52, 180)))):
         out = run(x[whole], ids[whole], weights[whole])
         for rows in parts:
