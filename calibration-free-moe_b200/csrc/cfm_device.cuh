@@ -253,9 +253,15 @@ __device__ __forceinline__ int cluster_size() {
 __device__ __forceinline__ void cluster_meet() {
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
+__device__ __forceinline__ void cluster_arrive() {
+  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void cluster_wait() {
+  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
 // What lies at this place of another CTA's shared memory.
 template <typename V>
-__device__ __forceinline__ const V* of_rank(const V* mine, int rank) {
+__device__ __forceinline__ V* of_rank(V* mine, int rank) {
   V* other;
   asm("mapa.u64 %0, %1, %2;" : "=l"(other) : "l"(mine), "r"(rank));
   return other;

@@ -248,8 +248,8 @@ __global__ void __launch_bounds__(kFewUpThreads, kFewUpPerSm)
   const int steps = (L.H / kFewUpBlock - warp + kFewUpWarps - 1) / kFewUpWarps * kPer, at = kFewUpBlock * warp + 8 * t, tiles = L.I / 8;
   auto column = [](int step) { return step / kPer * (kFewUpWarps * kFewUpBlock) + step % kPer * 32; };
   const FewGroups groups(routes, L.K, L.E);
-  Few few;
-  int count, c0, pass, pair;
+  Few few = {};
+  int count = 0, c0 = 0, pass = 0, pair = -1;
   const __nv_bfloat16 *gate, *up, *x;
   uint4 a[kFewUpAhead], b[kFewUpAhead], v[kFewUpAhead];
   auto fetch = [&](int i, int step) {

@@ -20,6 +20,8 @@ typedef unsigned long long u64;
 
 constexpr float kLog2E = 1.44269504f;
 constexpr float kInfinity = __builtin_huge_valf();
+// Stands for -inf where sums want a finite number: beside a largest value of up to kModerate its exponential is zero.
+constexpr float kLeast = -1e30f, kModerate = 1e29f;
 
 // 2^x, two units in the last place; 0 below -126.
 __device__ __forceinline__ float exp2_fast(float x) {
@@ -65,8 +67,9 @@ __device__ __forceinline__ u64 warp_max(u64 v) {
   return v;
 }
 
-// The warp's values in descending order.
-__device__ __forceinline__ u64 warp_sort(u64 v, int lane) {
+// The warp's values in descending order.  (Not inlined, as other parts that run once or twice per CTA are not: code that
+// is met for the first time comes from L2, and that was half of a call of one token.)
+__device__ __noinline__ u64 warp_sort(u64 v, int lane) {
 #pragma unroll
   for (int size = 2; size <= 32; size <<= 1)
 #pragma unroll
@@ -80,7 +83,7 @@ __device__ __forceinline__ u64 warp_sort(u64 v, int lane) {
 }
 // The largest 32 of two lists in descending order, in descending order: of a list and the other one
 // backwards the larger ones are those, as a bitonic sequence.
-__device__ __forceinline__ u64 warp_merge(u64 a, u64 b, int lane) {
+__device__ __noinline__ u64 warp_merge(u64 a, u64 b, int lane) {
   u64 v = max(a, __shfl_sync(kFull, b, 31 - lane));
 #pragma unroll
   for (int w = 16; w; w >>= 1) {
@@ -105,6 +108,26 @@ struct Element<__nv_bfloat16> {
       x[2 * i + 1] = bf16_hi(w[i]);
     }
   }
+  // Largest value of pieces, NaN if one is.
+  using Top = uint32_t;
+  static constexpr uint32_t kNone = 0xff80ff80u;
+  __device__ static Top lowest() { return kNone; }
+  __device__ static void fold(Top& top, const uint4& v) {
+    asm("max.NaN.bf16x2 %0, %0, %1;" : "+r"(top) : "r"(v.x));
+    asm("max.NaN.bf16x2 %0, %0, %1;" : "+r"(top) : "r"(v.y));
+    asm("max.NaN.bf16x2 %0, %0, %1;" : "+r"(top) : "r"(v.z));
+    asm("max.NaN.bf16x2 %0, %0, %1;" : "+r"(top) : "r"(v.w));
+  }
+  __device__ static float value(Top top) { return max_nan(bf16_lo(top), bf16_hi(top)); }
+  // With -inf (and NaN) raised to kLeast.
+  __device__ static void widen_bounded(uint4 v, float* x) {
+    constexpr uint32_t least = 0xf149f149u;  // twice, rounded down
+    asm("max.bf16x2 %0, %0, %1;" : "+r"(v.x) : "r"(least));
+    asm("max.bf16x2 %0, %0, %1;" : "+r"(v.y) : "r"(least));
+    asm("max.bf16x2 %0, %0, %1;" : "+r"(v.z) : "r"(least));
+    asm("max.bf16x2 %0, %0, %1;" : "+r"(v.w) : "r"(least));
+    widen(v, x);
+  }
   __device__ static float largest(const uint4& v) {
     uint32_t a, b;
     asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(a) : "r"(v.x), "r"(v.y));
@@ -126,6 +149,24 @@ struct Element<__half> {
       x[2 * i + 1] = f.y;
     }
   }
+  using Top = uint32_t;
+  static constexpr uint32_t kNone = 0xfc00fc00u;
+  __device__ static Top lowest() { return kNone; }
+  __device__ static void fold(Top& top, const uint4& v) {
+    asm("max.NaN.f16x2 %0, %0, %1;" : "+r"(top) : "r"(v.x));
+    asm("max.NaN.f16x2 %0, %0, %1;" : "+r"(top) : "r"(v.y));
+    asm("max.NaN.f16x2 %0, %0, %1;" : "+r"(top) : "r"(v.z));
+    asm("max.NaN.f16x2 %0, %0, %1;" : "+r"(top) : "r"(v.w));
+  }
+  __device__ static float value(Top top) {
+    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&top));
+    return max_nan(f.x, f.y);
+  }
+  __device__ static void widen_bounded(const uint4& v, float* x) {
+    widen(v, x);
+#pragma unroll
+    for (int i = 0; i < kWidth; ++i) x[i] = fmaxf(x[i], kLeast);
+  }
   __device__ static float largest(const uint4& v) {
     uint32_t a, b;
     asm("max.NaN.f16x2 %0, %1, %2;" : "=r"(a) : "r"(v.x), "r"(v.y));
@@ -144,6 +185,16 @@ struct Element<float> {
     x[1] = __uint_as_float(v.y);
     x[2] = __uint_as_float(v.z);
     x[3] = __uint_as_float(v.w);
+  }
+  using Top = float;
+  static constexpr uint32_t kNone = 0xff800000u;
+  __device__ static Top lowest() { return -kInfinity; }
+  __device__ static void fold(Top& top, const uint4& v) { top = max_nan(top, largest(v)); }
+  __device__ static float value(Top top) { return top; }
+  __device__ static void widen_bounded(const uint4& v, float* x) {
+    widen(v, x);
+#pragma unroll
+    for (int i = 0; i < kWidth; ++i) x[i] = fmaxf(x[i], kLeast);
   }
   __device__ static float largest(const uint4& v) {
     return max_nan(max_nan(__uint_as_float(v.x), __uint_as_float(v.y)),
@@ -175,40 +226,19 @@ struct Row {
   }
   // -inf stands where the row has nothing.
   __device__ uint4 load(int piece) const {
-    const int at = first(piece);
-    if (whole(piece)) return __ldg(reinterpret_cast<const uint4*>(data + at));
+    if (whole(piece)) return __ldg(reinterpret_cast<const uint4*>(data + first(piece)));
+    return load_edge(data, first(piece), columns);
+  }
+  __device__ __noinline__ static uint4 load_edge(const T* data, int at, int columns) {
     union {
       T e[W];
       uint4 v;
     } u;
-    T none;
-    if constexpr (sizeof(T) == 4) none = -kInfinity;
-    else if constexpr (std::is_same<T, __half>::value) none = __ushort_as_half(0xfc00);
-    else none = __ushort_as_bfloat16(0xff80);
+    u.v = make_uint4(Element<T>::kNone, Element<T>::kNone, Element<T>::kNone, Element<T>::kNone);
 #pragma unroll
-    for (int i = 0; i < W; ++i) u.e[i] = at + i >= 0 && at + i < columns ? data[at + i] : none;
-    return u.v;
-  }
-  // The largest element of a piece of which `value` is the largest value, with its place.
-  __device__ u64 find(int piece, float value) const {
-    const uint32_t key = ordered(value);
-    const int at = first(piece);
     for (int i = 0; i < W; ++i)
-      if (at + i >= 0 && at + i < columns && ordered(Element<T>::one(data + at + i)) == key)
-        return static_cast<u64>(key) << 32 | static_cast<uint32_t>(~(at + i));
-    return 0;
-  }
-};
-
-// Largest value that a thread has seen, and the first piece that has it.
-struct Best {
-  float value = -kInfinity;
-  int piece = -1;
-  __device__ void see(float v, int p) {
-    if (piece < 0 || (!(v <= value) && value == value)) {
-      value = v;
-      piece = p;
-    }
+      if (at + i >= 0 && at + i < columns) u.e[i] = data[at + i];
+    return u.v;
   }
 };
 
@@ -279,11 +309,24 @@ __global__ void __launch_bounds__(32 * kRouteRows)
 }
 
 // ---- log probabilities -----------------------------------------------------------------------------
-constexpr int kScoreThreads = 512;
+constexpr int kScoreThreads = 256;
 constexpr int kScoreWarps = kScoreThreads / 32;
-constexpr int kScoreAhead = 4;  // pieces of a thread that are on their way together
+constexpr int kScorePerSm = 4;
+constexpr int kScorePieces = 5;                 // of a thread that are added up together
+constexpr int kScoreRing = 2 * kScorePieces;    // that are on their way or kept
+constexpr size_t kRingBytes = static_cast<size_t>(kScoreThreads) * kScoreRing * 16;
+constexpr int kFound = 512;
+constexpr int kChunksKnown = 64;                // whose largest values the second pass looks at
 constexpr int kMaxTop = 32;
-constexpr int kMaxCluster = 8;
+constexpr int kMaxCluster = 16;
+
+// A thread's pieces of a row in shared memory, which it alone writes and reads.
+__device__ __forceinline__ uint32_t ring_slot(uint32_t ring, int slot) {
+  return ring + (slot * kScoreThreads + threadIdx.x) * 16;
+}
+__device__ __forceinline__ void store_shared16(uint32_t address, const uint4& v) {
+  asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(address), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
+}
 
 // Sums over elements x with the largest m: e^(x - m) without the `equal` elements that are m, and
 // e^(x - m) (x - m).  Without them the sum keeps its digits where one token has nearly all probability:
@@ -292,100 +335,173 @@ struct Sums {
   float m, equal, others, weighted;
 };
 
-// Tops of all warps' descending lists of 32, in the warps' first list; all threads.
-__device__ __forceinline__ void merge_lists(u64 (*lists)[32], int count, int warp, int lane) {
+// The sums of a lane's elements and of the other lanes', 2 * width of them, brought to one shift; every one of
+// those lanes has it.
+__device__ __noinline__ Sums sums_of_lanes(Sums s, int width) {
+  float m = s.m;
+  for (int w = width; w; w >>= 1) m = max_nan(m, __shfl_xor_sync(kFull, m, w));
+  if (s.m != m) {  // -inf: has seen nothing else
+    const float step = s.m - m, f = s.m > -kInfinity ? exp_fast(step) : 0.0f, all = s.others + s.equal;
+    s.weighted = f > 0.0f ? f * (s.weighted + step * all) : 0.0f;
+    s.others = f * all;
+    s.equal = 0.0f;
+    s.m = m;
+  }
+  for (int w = width; w; w >>= 1) {
+    s.equal += __shfl_xor_sync(kFull, s.equal, w);
+    s.others += __shfl_xor_sync(kFull, s.others, w);
+    s.weighted += __shfl_xor_sync(kFull, s.weighted, w);
+  }
+  return s;
+}
+
+// Tops of `count` descending lists of 32, twice the warps at most, in the first list; all threads.
+__device__ __noinline__ void merge_lists(u64 (*lists)[32], int count, int warp, int lane) {
   for (int step = 1; step < count; step <<= 1) {
     __syncthreads();
-    if (warp % (2 * step) == 0 && warp + step < count)
-      lists[warp][lane] = warp_merge(lists[warp][lane], lists[warp + step][lane], lane);
+    const int to = 2 * step * warp;
+    if (to + step < count) lists[to][lane] = warp_merge(lists[to][lane], lists[to + step][lane], lane);
   }
   __syncthreads();
 }
 
-// One cluster per row; its CTAs share the row's pieces.  One pass over the row gives the sums: per warp,
-// with the warp's largest value so far as the shift.  The top alternatives take a second pass, from the
-// caches: the n-th largest of the threads' own maxima is not above the n-th largest element, so few elements
-// are as large; those are sorted.  At most n threads have an element that large, which bounds their number
-// for every input.
+// One cluster per row; its CTAs share the row's pieces and hand their results to the first one.  One pass over the
+// row gives the sums: per warp, with the warp's largest value so far as the shift.  The top alternatives take a second
+// pass, from shared memory where the CTA's pieces fit the ring, else from the caches: the n-th largest of the
+// threads' own maxima is not above the n-th largest element, so few elements are as large; those are sorted.  Should
+// more than kFound be, the n-th largest of the first ones is a closer bound, and the pass is taken again: each time all but
+// n of those are out.
 template <typename T>
-__global__ void __launch_bounds__(kScoreThreads, 2)
-    k_token_logprobs(const void* logits, int64_t stride, int V, const void* tokens, int tokens64, int n,
-                     float* logprobs, float* entropy, int32_t* top_ids, float* top_logprobs) {
+__global__ void __launch_bounds__(kScoreThreads, kScorePerSm)
+    k_token_logprobs(const void* logits, int64_t stride, int V, const void* tokens, int tokens64, int n, float* logprobs,
+                     float* entropy, int32_t* top_ids, float* top_logprobs) {
   using E = Element<T>;
   constexpr int W = E::kWidth;
-  extern __shared__ u64 found[];
-  __shared__ u64 lists[kScoreWarps][32];
-  __shared__ Sums sums[kScoreWarps];
-  __shared__ double s_log_z;
-  __shared__ float s_m;
+  extern __shared__ __align__(16) uint8_t score_shared[];
+  __shared__ u64 found[kFound], lists[kScoreWarps][32], ranked[kMaxCluster][32];
+  __shared__ Sums sums[kScoreWarps], ranks_sums[kMaxCluster];
+  __shared__ float s_log_z, s_m, chunk_tops[kScoreWarps][kChunksKnown];
   __shared__ int s_found;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int ranks = cluster_size(), rank = cluster_rank();
   const int64_t r = blockIdx.x / ranks;
+  const uint32_t ring = shared_u32(score_shared);
+  cluster_arrive();
   grid_dependency_wait();
   grid_dependency_release();
   const Row<T> row(logits, stride, r, V);
   const int pieces = row.pieces();
   const int begin = static_cast<int>(static_cast<int64_t>(pieces) * rank / ranks);
   const int end = static_cast<int>(static_cast<int64_t>(pieces) * (rank + 1) / ranks);
-
-  Best best;
-  float m = -kInfinity, equal = 0.0f, others = 0.0f, weighted = 0.0f;
-  uint4 next[kScoreAhead];
+  const bool kept = end - begin <= kScoreRing * kScoreThreads;
+  // The thread's pieces are begin + tid, + 256, ...; a chunk is kScorePieces of them, of every thread.  -inf where it
+  // has no more.
+  constexpr int kChunk = kScorePieces * kScoreThreads;
+  const int whole_from = row.whole(0) ? 0 : 1, whole_to = row.whole(pieces - 1) ? pieces : pieces - 1;
+  auto bring_chunk = [&](int first, int slot) {
+    if (first >= whole_from && first + kChunk <= min(end, whole_to)) {
+      const T* from = row.data + row.first(first + tid);
 #pragma unroll
-  for (int j = 0; j < kScoreAhead; ++j) {
-    const int p = begin + tid + j * kScoreThreads;
-    if (p < end) next[j] = row.load(p);
-  }
-  for (int first = begin; first < end; first += kScoreAhead * kScoreThreads) {
-    uint4 v[kScoreAhead];
-    float top[kScoreAhead], chunk = -kInfinity;
-#pragma unroll
-    for (int j = 0; j < kScoreAhead; ++j) {
-      v[j] = next[j];
-      const int p = first + tid + j * kScoreThreads;
-      top[j] = -kInfinity;
-      if (p < end) {
-        top[j] = E::largest(v[j]);
-        best.see(top[j], p);
-        chunk = max_nan(chunk, top[j]);
+      for (int j = 0; j < kScorePieces; ++j) copy_async16(ring_slot(ring, slot + j), from + j * kScoreThreads * W);
+    } else {
+#pragma unroll 1
+      for (int j = 0; j < kScorePieces; ++j) {
+        const int p = first + tid + j * kScoreThreads;
+        if (p < end && row.whole(p)) copy_async16(ring_slot(ring, slot + j), row.data + row.first(p));
+        else store_shared16(ring_slot(ring, slot + j), p < end ? row.load(p) : make_uint4(E::kNone, E::kNone, E::kNone, E::kNone));
       }
-      const int ahead = p + kScoreAhead * kScoreThreads;
-      if (ahead < end) next[j] = row.load(ahead);
     }
-    chunk = warp_max_nan(chunk);
+    copy_async_commit();
+  };
+  bring_chunk(begin, 0);
+  bring_chunk(begin + kChunk, kScorePieces);
+  int64_t token = -1;
+  if (rank == 0 && tid == 0)
+    token = tokens64 ? static_cast<const int64_t*>(tokens)[r] : static_cast<const int32_t*>(tokens)[r];
+
+  float best = -kInfinity;  // of the thread, NaN above all, and the first chunk that has it
+  int best_chunk = begin;
+  float m = -kInfinity, equal = 0.0f, others = 0.0f, weighted = 0.0f;
+  int slot = 0, number = 0;
+  for (int first = begin; first < end; first += kChunk, slot = kScorePieces - slot, ++number) {
+    copy_async_wait<1>();
+    uint4 v[kScorePieces];
+    typename E::Top highest = E::lowest();
+#pragma unroll
+    for (int j = 0; j < kScorePieces; ++j) {
+      v[j] = load_shared16(ring_slot(ring, slot + j));
+      E::fold(highest, v[j]);
+    }
+    const float top = E::value(highest);
+    if (!kept) bring_chunk(first + 2 * kChunk, slot);
+    else copy_async_commit();
+    if (!(top <= best) && best == best) {
+      best = top;
+      best_chunk = first;
+    }
+    const float chunk = warp_max_nan(top);
+    if (lane == 0 && number < kChunksKnown) chunk_tops[warp][number] = chunk;
     if (!(chunk <= m) && m == m) {  // a new shift, the same in the whole warp; NaN stays
       const float step = m - chunk, f = m == -kInfinity ? 0.0f : exp_fast(step);
       const float all = others + equal;
-      weighted = m == -kInfinity ? 0.0f : f * (weighted + step * all);
+      weighted = f > 0.0f ? f * (weighted + step * all) : 0.0f;
       others = f * all;
       equal = 0.0f;
       m = chunk;
     }
     if (m == -kInfinity) continue;  // nothing but -inf so far
+    if (fabsf(m) <= kModerate) {
+      // In powers of two, from one multiply-add per element: 2^t, t = x log2 e - c, c = m log2 e as it rounds.
+      // m itself has t = t_m, next to zero; with that the chunk's sums are brought to the shift m.
+      const float c = __fmul_rn(m, kLog2E), t_m = __fmaf_rn(m, kLog2E, -c);
+      const Pair scale = pair_of(kLog2E, kLog2E), shift = pair_of(-c, -c);
+      Pair sum = pair_of(0.0f, 0.0f), moment = sum;
 #pragma unroll
-    for (int j = 0; j < kScoreAhead; ++j) {
-      if (top[j] == -kInfinity) continue;
-      float x[W];
-      E::widen(v[j], x);
-      if (top[j] == m) {
+      for (int j = 0; j < kScorePieces; ++j) {
+        float x[W];
+        E::widen_bounded(v[j], x);
+        if (top == m) {
 #pragma unroll
-        for (int i = 0; i < W; ++i)
-          if (x[i] == m) {
-            equal += 1.0f;
-            x[i] = -kInfinity;
-          }
+          for (int i = 0; i < W; ++i)
+            if (x[i] == m) {
+              equal += 1.0f;
+              x[i] = kLeast;
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < W; i += 2) {
+          const Pair t = pair_fma(pair_of(x[i], x[i + 1]), scale, shift);
+          float t0, t1;
+          pair_split(t, t0, t1);
+          const Pair e = pair_of(exp2_fast(t0), exp2_fast(t1));
+          sum = pair_add(sum, e);
+          moment = pair_fma(e, t, moment);
+        }
       }
+      float s0, s1, w0, w1;
+      pair_split(sum, s0, s1);
+      pair_split(moment, w0, w1);
+      const float back = exp2_fast(-t_m), all = s0 + s1;
+      others = __fmaf_rn(all, back, others);
+      weighted = __fmaf_rn(0.693147181f * back, (w0 + w1) - t_m * all, weighted);
+      continue;
+    }
+#pragma unroll 1
+    for (int p = first + tid; p < min(end, first + kChunk); p += kScoreThreads) {  // values beyond 10^29, or NaN, which the shift tells of
+      float x[W];
+      E::widen(row.load(p), x);
 #pragma unroll
       for (int i = 0; i < W; ++i) {
-        const float d = fmaxf(__fsub_rn(x[i], m), -1e30f);  // -inf: adds nothing
+        const float d = x[i] == m ? kLeast : fmaxf(__fsub_rn(x[i], m), kLeast);  // -inf: adds nothing
         const float e = exp_fast(d);
+        equal += x[i] == m;
         others += e;
         weighted = __fmaf_rn(e, d, weighted);
       }
     }
   }
-  // NaN does not reach the sums by fmaxf: the shift says so.
+  const bool given = token >= 0 && token < V;
+  const float x_token = given ? E::one(row.data + token) : 0.0f;
 #pragma unroll
   for (int w = 16; w; w >>= 1) {
     equal += __shfl_xor_sync(kFull, equal, w);
@@ -396,257 +512,499 @@ __global__ void __launch_bounds__(kScoreThreads, 2)
 
   if (n) {
     // The thread's largest element, NaN above all.
-    u64 top = best.piece >= 0 ? row.find(best.piece, best.value) : 0;
-    lists[warp][lane] = warp_sort(top, lane);
-    if (tid == 0) s_found = 0;
-    merge_lists(lists, kScoreWarps, warp, lane);
-    const u64 least = lists[0][n - 1];  // 0: fewer threads than n have elements, all of them are taken
-    const float floor = value_of(static_cast<uint32_t>(least >> 32));
-    for (int p = begin + tid; p < end; p += kScoreThreads) {
-      const uint4 v = row.load(p);
-      if (least && E::largest(v) < floor) continue;
+    auto again = [&](int p) { return kept ? load_shared16(ring_slot(ring, (p - begin) / kScoreThreads)) : row.load(p); };
+    int best_piece = -1;
+#pragma unroll 1
+    for (int p = best_chunk + tid; p < min(end, best_chunk + kChunk) && best_piece < 0; p += kScoreThreads) {
+      const float highest = E::largest(again(p));
+      if (highest == best || (highest != highest && best != best)) best_piece = p;
+    }
+    u64 top = 0;
+    if (best_piece >= 0) {
       float x[W];
-      E::widen(v, x);
-      const int at = row.first(p);
+      E::widen(again(best_piece), x);
+      const int at = row.first(best_piece);
 #pragma unroll
-      for (int i = 0; i < W; ++i) {
-        if (at + i < 0 || at + i >= V) continue;
-        const u64 key = placed(x[i], at + i);
-        if (key >= least) found[atomicAdd(&s_found, 1)] = key;
-      }
+      for (int i = 0; i < W; ++i)
+        if (at + i >= 0 && at + i < V) top = max(top, placed(x[i], at + i));
     }
-    __syncthreads();
-    const int count = s_found;
-    u64 list = 0;
-    for (int i = 32 * warp; i < count; i += kScoreThreads) {
-      const u64 more = warp_sort(i + lane < count ? found[i + lane] : 0, lane);
-      list = i == 32 * warp ? more : warp_merge(list, more, lane);
-    }
-    lists[warp][lane] = list;
+    lists[warp][lane] = warp_sort(top, lane);
     merge_lists(lists, kScoreWarps, warp, lane);
-  }
-  __syncthreads();
-  cluster_meet();
-  if (rank == 0) {
-    if (warp == 0) {
-      const int entries = ranks * kScoreWarps;
-      float largest = -kInfinity;
-      for (int i = lane; i < entries; i += 32)
-        largest = max_nan(largest, of_rank(&sums[i % kScoreWarps], i / kScoreWarps)->m);
-      largest = warp_max_nan(largest);
-      double equals = 0.0, rest = 0.0, total = 0.0;
-      for (int i = lane; i < entries; i += 32) {
-        const Sums s = *of_rank(&sums[i % kScoreWarps], i / kScoreWarps);
-        if (s.m == largest) {
-          equals += s.equal;
-          rest += s.others;
-          total += s.weighted;
-        } else if (s.m > -kInfinity) {
-          const float step = s.m - largest, f = expf(step);
-          rest += f * (s.others + s.equal);
-          total += f * (s.weighted + step * (s.others + s.equal));
+    while (true) {
+      const u64 least = lists[0][n - 1];  // 0: fewer threads than n have elements
+      const float floor = value_of(static_cast<uint32_t>(least >> 32));
+      if (tid == 0) s_found = 0;
+      __syncthreads();
+      int chunk = 0;
+      for (int first = begin; first < end; first += kChunk, ++chunk) {
+        if (least && chunk < kChunksKnown && chunk_tops[warp][chunk] < floor) continue;
+        // Pieces that have one, then those one after another.
+        unsigned has = 0;
+#pragma unroll
+        for (int j = 0; j < kScorePieces; ++j) {
+          const int p = first + tid + j * kScoreThreads;
+          if (p < end && !(least && E::largest(again(p)) < floor)) has |= 1u << j;
+        }
+        while (has) {
+          const int p = first + tid + (__ffs(has) - 1) * kScoreThreads, at = row.first(p);
+          has &= has - 1;
+          float x[W];
+          E::widen(again(p), x);
+#pragma unroll
+          for (int i = 0; i < W; ++i) {
+            if ((least && x[i] < floor) || at + i < 0 || at + i >= V) continue;
+            const u64 key = placed(x[i], at + i);
+            if (key < least) continue;
+            const int place = atomicAdd(&s_found, 1);
+            if (place < kFound) found[place] = key;
+          }
         }
       }
-#pragma unroll
-      for (int w = 16; w; w >>= 1) {
-        equals += __shfl_xor_sync(kFull, equals, w);
-        rest += __shfl_xor_sync(kFull, rest, w);
-        total += __shfl_xor_sync(kFull, total, w);
-      }
-      if (lane == 0) {
-        // A row of nothing but -inf, with NaN or with +inf has no distribution.
-        const bool none = !(fabsf(largest) < kInfinity);
-        const double nan = __longlong_as_double(0x7fffffffffffffffll);
-        const double log_z = none ? nan : log1p(rest + (equals - 1.0));
-        const int64_t token = tokens64 ? static_cast<const int64_t*>(tokens)[r] : static_cast<const int32_t*>(tokens)[r];
-        const bool given = token >= 0 && token < V;
-        const float x = given ? E::one(row.data + token) : 0.0f;
-        logprobs[r] = static_cast<float>(given && !none ? static_cast<double>(x - largest) - log_z : nan);
-        entropy[r] = static_cast<float>(none ? nan : log_z - total / (rest + equals));
-        s_log_z = log_z;
-        s_m = largest;
-      }
-    }
-    if (n) {
       __syncthreads();
-      if (warp < ranks && warp > 0) lists[warp][lane] = of_rank(&lists[0][0], warp)[lane];
-      merge_lists(lists, ranks, warp, lane);
-      if (tid < n) {
-        const u64 key = lists[0][lane];
-        const int64_t at = r * n + tid;
-        top_ids[at] = place_of(key);
-        top_logprobs[at] = static_cast<float>(static_cast<double>(value_of(static_cast<uint32_t>(key >> 32)) - s_m) - s_log_z);
+      const int all = s_found, count = min(all, kFound);
+      u64 list = 0;
+      for (int i = 32 * warp; i < count; i += kScoreThreads) {
+        const u64 more = warp_sort(i + lane < count ? found[i + lane] : 0, lane);
+        list = i == 32 * warp ? more : warp_merge(list, more, lane);
       }
+      lists[warp][lane] = list;
+      merge_lists(lists, min(kScoreWarps, (count + 31) / 32), warp, lane);
+      if (all <= kFound) break;
+    }
+  } else {
+    __syncthreads();
+  }
+  // To the first CTA; the others are done then.
+  cluster_wait();  // it has started
+  if (warp == 0) {
+    const Sums mine = sums_of_lanes(lane < kScoreWarps ? sums[lane] : Sums{-kInfinity, 0.0f, 0.0f, 0.0f}, 16);
+    if (lane == 0) *of_rank(&ranks_sums[rank], 0) = mine;
+  } else if (warp == 1 && n) {
+    of_rank(&ranked[rank][0], 0)[lane] = lists[0][lane];
+  }
+  cluster_arrive();
+  if (rank) return;
+  cluster_wait();
+  if (warp == 0) {
+    const Sums all = sums_of_lanes(lane < ranks ? ranks_sums[lane] : Sums{-kInfinity, 0.0f, 0.0f, 0.0f}, kMaxCluster / 2);
+    if (lane == 0) {
+      // A row of nothing but -inf, with NaN or with +inf has no distribution.
+      const bool none = !(fabsf(all.m) < kInfinity);
+      const float nan = __int_as_float(0x7fffffff);
+      const float log_z = none ? nan : log1pf(all.others + (all.equal - 1.0f));
+      logprobs[r] = given ? (x_token - all.m) - log_z : nan;
+      entropy[r] = log_z - all.weighted / (all.others + all.equal);
+      s_log_z = log_z;
+      s_m = all.m;
     }
   }
-  cluster_meet();  // the others' shared memory has been read
+  if (n) {
+    merge_lists(ranked, ranks, warp, lane);
+    if (tid < n) {
+      const u64 key = ranked[0][lane];
+      const int64_t at = r * n + tid;
+      top_ids[at] = place_of(key);
+      top_logprobs[at] = (value_of(static_cast<uint32_t>(key >> 32)) - s_m) - s_log_z;
+    }
+  }
 }
 
 // ---- divergence ------------------------------------------------------------------------------------
-// (e^-t - 1 + t) / t^2 for |t| up to 1/2, from the series: the first term left out is 4e-8 of the sum.
-__device__ __forceinline__ float remainder_series(float t) {
-  float p = 1.0f / 40320.0f;
-  p = __fmaf_rn(p, t, -1.0f / 5040.0f);
-  p = __fmaf_rn(p, t, 1.0f / 720.0f);
+// KL(P || Q) = E[d] + log E[e^-d] over P, d = a - b.  With any shift taken from d, t = d - shift,
+// psi(t) = e^-t - 1 + t and x = E[psi] - E[t], it is
+//   E[psi] + (log1p(x) - x),
+// where nothing of first order in t is left to cancel: rows that hardly differ keep their digits in FP32.
+// A shift is changed by D without loss: psi(t + D) = e^-D psi(t) + psi(D) - (e^-D - 1) t.
+constexpr int kComparePieces = 3;  // of a thread and row that are looked at together
+constexpr int kCompareChunk = kComparePieces * kScoreThreads;
+constexpr size_t kCompareRing = 4ull * kComparePieces * kScoreThreads * 16;  // two chunks of two rows
+constexpr float kNear = 60.0f;     // |t| of the single pass; beyond, and where a row has -inf alone, NaN or +inf, there is another
+
+// psi(t) / t^2 for |t| up to 1/2: the series to t^6, whose last term the Chebyshev polynomial of degree six turns into
+// lower ones; 3e-8 of the value.
+__device__ __forceinline__ float psi_series(float t) {
+  constexpr float last = 1.0f / 40320.0f;
+  float p = -1.0f / 5040.0f;
+  p = __fmaf_rn(p, t, 1.0f / 720.0f + 0.375f * last);
   p = __fmaf_rn(p, t, -1.0f / 120.0f);
-  p = __fmaf_rn(p, t, 1.0f / 24.0f);
+  p = __fmaf_rn(p, t, 1.0f / 24.0f - 0.03515625f * last);
   p = __fmaf_rn(p, t, -1.0f / 6.0f);
-  return __fmaf_rn(p, t, 0.5f);
+  return __fmaf_rn(p, t, 0.5f + 0.00048828125f * last);
+}
+__device__ __forceinline__ float psi(float t) {
+  return fabsf(t) <= 0.5f ? __fmul_rn(__fmul_rn(t, t), psi_series(t)) : (exp_fast(-t) - 1.0f) + t;
 }
 
-// Over a row, with e = e^(a - max a): sums of e, of e t and of e (e^-t - 1 + t); or, where the rows are far
-// apart, of e, of e t and of e^(b - max b).
+// Of some elements, with e = e^(a - m): sums of e, e t and e psi(t); whether the single pass does not hold for them.
 struct Moments {
-  float mass, shift, remainder;
-  int infinite;
+  float m, shift, mass, mean, rest;
+  int beyond;
 };
 
-// One cluster per row; its CTAs share the row's pieces.  KL(P || Q) = E[d] + log E[e^-d] over P, d = a - b.
-// With any shift taken from d, t = d - shift, and x = E[e^-t - 1 + t] - E[t], it is
-//   E[e^-t - 1 + t] + (log1p(x) - x),
-// where nothing of first order in t is left to cancel: rows that hardly differ keep their digits in FP32.
-// The shift is d at the largest a, so the row's maxima are found first; the second pass reads from the caches.
-// An element of which P has nothing adds its e^(b - b*) there, for the sum of all of them is Q's.
+// The same of another shift of t.
+__device__ __forceinline__ void reshift(Moments& s, float shift) {
+  const float by = __fsub_rn(s.shift, shift);
+  if (!(fabsf(by) <= kNear)) s.beyond = 1;
+  const float more = psi(by), less = fabsf(by) <= 0.5f ? __fsub_rn(more, by) : exp_fast(-by) - 1.0f;  // e^-by - 1
+  s.rest = s.rest + (less * (s.rest - s.mean) + more * s.mass);
+  s.mean = __fmaf_rn(by, s.mass, s.mean);
+  s.shift = shift;
+}
+
+// The lanes' moments as one, in every lane, with the shift of a lane that has the largest a: where nearly all of the
+// mass is on one element, t is zero there, and the small parts of the others are not lost beside it.
+__device__ __noinline__ Moments moments_of_lanes(Moments s) {
+  float m = s.m;
+#pragma unroll
+  for (int w = 16; w; w >>= 1) m = fmaxf(m, __shfl_xor_sync(kFull, m, w));
+  const bool has = s.mass > 0.0f;
+  const unsigned having = __ballot_sync(kFull, has && s.m == m);
+  const float shift = __shfl_sync(kFull, s.shift, having ? __ffs(having) - 1 : 0);
+  if (has) reshift(s, shift);
+  const float f = has ? exp_fast(__fsub_rn(s.m, m)) : 0.0f;
+  Moments all;
+  all.m = m;
+  all.shift = shift;
+  all.mass = f * s.mass;
+  all.mean = f * s.mean;
+  all.rest = f * s.rest;
+  all.beyond = s.beyond;
+#pragma unroll
+  for (int w = 16; w; w >>= 1) {
+    all.mass += __shfl_xor_sync(kFull, all.mass, w);
+    all.mean += __shfl_xor_sync(kFull, all.mean, w);
+    all.rest += __shfl_xor_sync(kFull, all.rest, w);
+    all.beyond |= __shfl_xor_sync(kFull, all.beyond, w);
+  }
+  return all;
+}
+
+// What a CTA has of its row.
+struct Compared {
+  Moments moments;
+  u64 tops[2];  // largest elements
+};
+
+// The largest elements of a thread's pieces of two rows' chunks of which `value` are the largest values, with their places;
+// a chunk that starts at `end` has none.
 template <typename T>
-__global__ void __launch_bounds__(kScoreThreads, 2)
+__device__ __noinline__ ulonglong2 largest_of_chunks(Row<T> a, Row<T> b, int2 first, int end, float2 value) {
+  using E = Element<T>;
+  constexpr int W = E::kWidth;
+  uint4 v[2][kComparePieces];
+#pragma unroll
+  for (int j = 0; j < kComparePieces; ++j) {
+    const int p = first.x + threadIdx.x + j * kScoreThreads, q = first.y + threadIdx.x + j * kScoreThreads;
+    if (p < end) v[0][j] = a.load(p);
+    if (q < end) v[1][j] = b.load(q);
+  }
+  int place[2] = {0x7fffffff, 0x7fffffff};
+#pragma unroll
+  for (int of = 0; of < 2; ++of)
+#pragma unroll
+    for (int j = 0; j < kComparePieces; ++j) {
+      const int p = (of ? first.y : first.x) + threadIdx.x + j * kScoreThreads;
+      if (p >= end) continue;
+      float x[W];
+      E::widen(v[of][j], x);
+      const int at = a.first(p);
+      const float most = of ? value.y : value.x;
+#pragma unroll
+      for (int i = 0; i < W; ++i)
+        if ((x[i] == most || (x[i] != x[i] && most != most)) && at + i >= 0 && at + i < a.columns) place[of] = min(place[of], at + i);
+    }
+  return make_ulonglong2(place[0] < 0x7fffffff ? placed(value.x, place[0]) : 0, place[1] < 0x7fffffff ? placed(value.y, place[1]) : 0);
+}
+
+// The other pass, over rows that are far apart or have -inf where the other has not: sums of e^(a - max a), of that
+// times t and, with `apart`, of e^(b - max b); else of e^(a - max a) psi(t), where an element of which P has nothing
+// adds its e^(b - b*), for the sum of all of those is Q's.  `infinite`: Q has nothing where P has something.
+template <typename T>
+__device__ __noinline__ Moments far_moments(Row<T> a, Row<T> b, int begin, int end, float most_a, float base_b,
+                                            bool apart) {
+  using E = Element<T>;
+  constexpr int W = E::kWidth;
+  Moments sum = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0};
+  const float shift = most_a - base_b;
+#pragma unroll 1
+  for (int p = begin + threadIdx.x; p < end; p += kScoreThreads) {
+    float x[W], y[W];
+    E::widen(a.load(p), x);
+    E::widen(b.load(p), y);
+#pragma unroll
+    for (int i = 0; i < W; ++i) {
+      const float t = __fsub_rn(__fsub_rn(x[i], y[i]), shift), size = fabsf(t);
+      const float e = x[i] > -kInfinity ? exp_fast(__fsub_rn(x[i], most_a)) : 0.0f;
+      if (x[i] > -kInfinity && y[i] == -kInfinity) sum.beyond = 1;
+      const float u = e > 0.0f ? __fmul_rn(e, t) : 0.0f, of_b = exp_fast(__fsub_rn(y[i], base_b));
+      sum.mass += e;
+      sum.mean += u;
+      sum.rest += apart ? of_b : size <= 16.0f ? __fmul_rn(e, psi(t)) : of_b - e + u;
+    }
+  }
+#pragma unroll
+  for (int w = 16; w; w >>= 1) {
+    sum.mass += __shfl_xor_sync(kFull, sum.mass, w);
+    sum.mean += __shfl_xor_sync(kFull, sum.mean, w);
+    sum.rest += __shfl_xor_sync(kFull, sum.rest, w);
+    sum.beyond |= __shfl_xor_sync(kFull, sum.beyond, w);
+  }
+  return sum;
+}
+
+// One cluster per row; its CTAs share the row's pieces.  One pass over both rows: a warp takes its largest a so far
+// as the exponentials' shift, and d at the largest a of its first elements as that of t.
+template <typename T>
+__global__ void __launch_bounds__(kScoreThreads, kScorePerSm)
     k_compare_logits(const void* reference, int64_t reference_stride, const void* logits, int64_t stride, int V,
                      float* divergence, uint8_t* agreement) {
   using E = Element<T>;
   constexpr int W = E::kWidth;
-  __shared__ u64 tops[2][kScoreWarps];
-  __shared__ u64 s_top[2];
+  extern __shared__ __align__(16) uint8_t compare_shared[];
+  __shared__ Compared compared;
   __shared__ Moments moments[kScoreWarps];
+  __shared__ u64 tops[2][kScoreWarps];
+  __shared__ float highs[2][kScoreWarps];
+  __shared__ int s_beyond;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int ranks = cluster_size(), rank = cluster_rank();
   const int64_t r = blockIdx.x / ranks;
+  const uint32_t ring = shared_u32(compare_shared);
   grid_dependency_wait();
   grid_dependency_release();
   const Row<T> a(reference, reference_stride, r, V), b(logits, stride, r, V, a.shift);
   const int pieces = a.pieces();
   const int begin = static_cast<int>(static_cast<int64_t>(pieces) * rank / ranks);
   const int end = static_cast<int>(static_cast<int64_t>(pieces) * (rank + 1) / ranks);
+  const int whole_from = a.whole(0) && b.whole(0) ? 0 : 1, whole_to = a.whole(pieces - 1) && b.whole(pieces - 1) ? pieces : pieces - 1;
+  // Slots of a chunk: the pieces of a, then those of b.  -inf where there are no more.
+  auto bring_chunk = [&](int first, int slot) {
+    if (first >= whole_from && first + kCompareChunk <= min(end, whole_to) && b.aligned) {
+      const T *x = a.data + a.first(first + tid), *y = b.data + b.first(first + tid);
+#pragma unroll
+      for (int j = 0; j < kComparePieces; ++j) {
+        copy_async16(ring_slot(ring, slot + j), x + j * kScoreThreads * W);
+        copy_async16(ring_slot(ring, slot + kComparePieces + j), y + j * kScoreThreads * W);
+      }
+    } else {
+#pragma unroll 1
+      for (int j = 0; j < kComparePieces; ++j) {
+        const int p = first + tid + j * kScoreThreads;
+        const uint4 none = make_uint4(E::kNone, E::kNone, E::kNone, E::kNone);
+        store_shared16(ring_slot(ring, slot + j), p < end ? a.load(p) : none);
+        store_shared16(ring_slot(ring, slot + kComparePieces + j), p < end ? b.load(p) : none);
+      }
+    }
+    copy_async_commit();
+  };
+  bring_chunk(begin, 0);
+  bring_chunk(begin + kCompareChunk, 2 * kComparePieces);
 
-  Best best_a, best_b;
-#pragma unroll 4
-  for (int p = begin + tid; p < end; p += kScoreThreads) {
-    const uint4 va = a.load(p), vb = b.load(p);
-    best_a.see(E::largest(va), p);
-    best_b.see(E::largest(vb), p);
-  }
-  const u64 top_a = warp_max(best_a.piece >= 0 ? a.find(best_a.piece, best_a.value) : 0);
-  const u64 top_b = warp_max(best_b.piece >= 0 ? b.find(best_b.piece, best_b.value) : 0);
-  if (lane == 0) {
-    tops[0][warp] = top_a;
-    tops[1][warp] = top_b;
-  }
-  __syncthreads();
-  cluster_meet();
-  if (warp < 2) {
-    u64 top = 0;
-    for (int i = lane; i < ranks * kScoreWarps; i += 32)
-      top = max(top, *of_rank(&tops[warp][i % kScoreWarps], i / kScoreWarps));
-    top = warp_max(top);
-    if (lane == 0) s_top[warp] = top;
-  }
-  __syncthreads();
-  const float most_a = value_of(static_cast<uint32_t>(s_top[0] >> 32));
-  const float most_b = value_of(static_cast<uint32_t>(s_top[1] >> 32));
-  const float b_there = E::one(b.data + place_of(s_top[0]));
-  // Rows without a distribution (nothing but -inf, with NaN or with +inf); rows so far apart that e^(b - b*) overflows.
-  const bool none = !(fabsf(most_a) < kInfinity) || !(fabsf(most_b) < kInfinity);
-  const bool far = !(most_b - b_there <= 60.0f);
-  const float base_b = far ? most_b : b_there, shift = most_a - base_b;
-
-  Moments sum = {0.0f, 0.0f, 0.0f, 0};
-  if (!none) {
-#pragma unroll 2
-    for (int p = begin + tid; p < end; p += kScoreThreads) {
-      float x[W], y[W], t[W], widest = 0.0f;
-      E::widen(a.load(p), x);
-      E::widen(b.load(p), y);
+  float best_a = -kInfinity, best_b = -kInfinity;  // of the thread, NaN above all, and the first chunks that have them
+  int chunk_a = begin, chunk_b = begin;
+  Moments sum = {-kInfinity, 0.0f, 0.0f, 0.0f, 0.0f, 0};
+  int slot = 0;
+  for (int first = begin; first < end; first += kCompareChunk, slot = 2 * kComparePieces - slot) {
+    copy_async_wait<1>();
+    typename E::Top high_a = E::lowest(), high_b = E::lowest();
 #pragma unroll
-      for (int i = 0; i < W; ++i) {
-        t[i] = __fsub_rn(__fsub_rn(x[i], y[i]), shift);
-        widest = max_nan(widest, fabsf(t[i]));
-      }
-      if (widest <= 0.5f && !far) {
+    for (int j = 0; j < kComparePieces; ++j) {
+      E::fold(high_a, load_shared16(ring_slot(ring, slot + j)));
+      E::fold(high_b, load_shared16(ring_slot(ring, slot + kComparePieces + j)));
+    }
+    const float top_a = E::value(high_a), top_b = E::value(high_b);
+    if (!(top_a <= best_a) && best_a == best_a) {
+      best_a = top_a;
+      chunk_a = first;
+    }
+    if (!(top_b <= best_b) && best_b == best_b) {
+      best_b = top_b;
+      chunk_b = first;
+    }
+    const float chunk = warp_max_nan(top_a);
+    // Too large to be scaled, or NaN.
+    if ((!(fabsf(chunk) <= kModerate) && chunk != -kInfinity) || top_b != top_b) sum.beyond = 1;
+    if (chunk > sum.m && chunk <= kModerate) {  // new shifts, the same in the whole warp: of its largest a
+      float d = 0.0f;
+      if (top_a == chunk) {
+#pragma unroll 1
+        for (int j = 0; j < kComparePieces; ++j) {
+          float x[W], y[W];
+          E::widen_bounded(load_shared16(ring_slot(ring, slot + j)), x);
+          E::widen_bounded(load_shared16(ring_slot(ring, slot + kComparePieces + j)), y);
 #pragma unroll
-        for (int i = 0; i < W; ++i) {
-          const float e = exp_fast(__fsub_rn(x[i], most_a)), u = __fmul_rn(e, t[i]);
-          sum.mass += e;
-          sum.shift += u;
-          sum.remainder = __fmaf_rn(__fmul_rn(u, t[i]), remainder_series(t[i]), sum.remainder);
+          for (int i = 0; i < W; ++i)
+            if (x[i] == chunk) d = __fsub_rn(x[i], y[i]);
         }
-        continue;
       }
+      d = __shfl_sync(kFull, d, __ffs(__ballot_sync(kFull, top_a == chunk)) - 1);
+      if (sum.m > -kInfinity) {
+        const float f = exp_fast(__fsub_rn(sum.m, chunk));
+        reshift(sum, d);
+        sum.mass *= f;
+        sum.mean *= f;
+        sum.rest *= f;
+      }
+      sum.shift = d;
+      sum.m = chunk;
+    }
+    if (fabsf(sum.m) <= kModerate) {
+      const float m = sum.m, shift = sum.shift;
+      const float c = __fmul_rn(m, kLog2E), back = exp2_fast(-__fmaf_rn(m, kLog2E, -c));
+      const Pair scale = pair_of(kLog2E, kLog2E), base = pair_of(-c, -c), minus = pair_of(-1.0f, -1.0f), less = pair_of(-shift, -shift);
+      Pair masses = pair_of(0.0f, 0.0f), means = masses, rests = masses;
+      float widest = 0.0f;
 #pragma unroll
-      for (int i = 0; i < W; ++i) {
-        const float e = x[i] > -kInfinity ? exp_fast(__fsub_rn(x[i], most_a)) : 0.0f;
-        if (x[i] > -kInfinity && y[i] == -kInfinity) sum.infinite = 1;
-        const float u = e > 0.0f ? __fmul_rn(e, t[i]) : 0.0f;
-        const float of_b = exp_fast(__fsub_rn(y[i], base_b));
-        float more = of_b;
-        if (!far) {
-          const float size = fabsf(t[i]);
-          more = size <= 0.5f    ? __fmul_rn(__fmul_rn(u, t[i]), remainder_series(t[i]))
-                 : size <= 16.0f ? __fmul_rn(e, exp_fast(-t[i]) - 1.0f + t[i])
-                                 : of_b - e + u;
+      for (int j = 0; j < kComparePieces; ++j) {
+        float x[W], y[W];
+        E::widen_bounded(load_shared16(ring_slot(ring, slot + j)), x);
+        E::widen_bounded(load_shared16(ring_slot(ring, slot + kComparePieces + j)), y);
+        Pair t[W / 2];
+        float wide = 0.0f;
+#pragma unroll
+        for (int i = 0; i < W / 2; ++i) {
+          t[i] = pair_add(pair_fma(pair_of(y[2 * i], y[2 * i + 1]), minus, pair_of(x[2 * i], x[2 * i + 1])), less);
+          float t0, t1;
+          pair_split(t[i], t0, t1);
+          wide = fmaxf(wide, fmaxf(fabsf(t0), fabsf(t1)));
         }
-        sum.mass += e;
-        sum.shift += u;
-        sum.remainder += more;
+        widest = fmaxf(widest, wide);
+        const bool small = wide <= 0.5f;
+#pragma unroll
+        for (int i = 0; i < W / 2; ++i) {
+          float p0, p1, t0, t1;
+          pair_split(pair_fma(pair_of(x[2 * i], x[2 * i + 1]), scale, base), p0, p1);
+          pair_split(t[i], t0, t1);
+          const Pair e = pair_of(exp2_fast(p0), exp2_fast(p1));
+          masses = pair_add(masses, e);
+          means = pair_fma(e, t[i], means);
+          Pair value = pair_mul(pair_mul(t[i], t[i]), pair_of(psi_series(t0), psi_series(t1)));
+          if (!small) {
+            float v0, v1;
+            pair_split(value, v0, v1);
+            value = pair_of(fabsf(t0) <= 0.5f ? v0 : (exp_fast(-t0) - 1.0f) + t0,
+                            fabsf(t1) <= 0.5f ? v1 : (exp_fast(-t1) - 1.0f) + t1);
+          }
+          rests = pair_fma(e, value, rests);
+        }
       }
+      if (!(widest <= kNear)) sum.beyond = 1;
+      float s0, s1;
+      pair_split(masses, s0, s1);
+      sum.mass = __fmaf_rn(s0 + s1, back, sum.mass);
+      pair_split(means, s0, s1);
+      sum.mean = __fmaf_rn(s0 + s1, back, sum.mean);
+      pair_split(rests, s0, s1);
+      sum.rest = __fmaf_rn(s0 + s1, back, sum.rest);
     }
+    bring_chunk(first + 2 * kCompareChunk, slot);
   }
-#pragma unroll
-  for (int w = 16; w; w >>= 1) {
-    sum.mass += __shfl_xor_sync(kFull, sum.mass, w);
-    sum.shift += __shfl_xor_sync(kFull, sum.shift, w);
-    sum.remainder += __shfl_xor_sync(kFull, sum.remainder, w);
-    sum.infinite |= __shfl_xor_sync(kFull, sum.infinite, w);
-  }
-  if (lane == 0) moments[warp] = sum;
-  __syncthreads();
-  cluster_meet();
-  if (rank == 0 && warp == 0) {
-    double mass = 0.0, mean = 0.0, rest = 0.0;
-    int infinite = 0;
-    for (int i = lane; i < ranks * kScoreWarps; i += 32) {
-      const Moments other = *of_rank(&moments[i % kScoreWarps], i / kScoreWarps);
-      mass += other.mass;
-      mean += other.shift;
-      rest += other.remainder;
-      infinite |= other.infinite;
-    }
-#pragma unroll
-    for (int w = 16; w; w >>= 1) {
-      mass += __shfl_xor_sync(kFull, mass, w);
-      mean += __shfl_xor_sync(kFull, mean, w);
-      rest += __shfl_xor_sync(kFull, rest, w);
-      infinite |= __shfl_xor_sync(kFull, infinite, w);
-    }
+  // The warps', the CTA's.
+  const float high_a = warp_max_nan(best_a), high_b = warp_max_nan(best_b);
+  {
+    const Moments all = moments_of_lanes(sum);
     if (lane == 0) {
-      double kl;
+      moments[warp] = all;
+      highs[0][warp] = high_a;
+      highs[1][warp] = high_b;
+      tops[0][warp] = tops[1][warp] = 0;
+    }
+  }
+  __syncthreads();
+  {
+    // The threads that have a largest value look for its place.
+    float most_a = highs[0][lane % kScoreWarps], most_b = highs[1][lane % kScoreWarps];
+    most_a = warp_max_nan(most_a);
+    most_b = warp_max_nan(most_b);
+    const bool has_a = best_a == most_a || (best_a != best_a && most_a != most_a);
+    const bool has_b = best_b == most_b || (best_b != best_b && most_b != most_b);
+    if (__any_sync(kFull, has_a || has_b)) {
+      const ulonglong2 found = largest_of_chunks(a, b, make_int2(has_a ? chunk_a : end, has_b ? chunk_b : end), end, make_float2(best_a, best_b));
+      const u64 top_a = warp_max(found.x), top_b = warp_max(found.y);
+      if (lane == 0) {
+        tops[0][warp] = top_a;
+        tops[1][warp] = top_b;
+      }
+    }
+  }
+  if (warp == 0) {
+    const Moments all = moments_of_lanes(lane < kScoreWarps ? moments[lane] : Moments{-kInfinity, 0.0f, 0.0f, 0.0f, 0.0f, 0});
+    if (lane == 0) compared.moments = all;
+  }
+  __syncthreads();
+  if (warp == 0) {
+    const u64 top_a = warp_max(lane < kScoreWarps ? tops[0][lane] : 0), top_b = warp_max(lane < kScoreWarps ? tops[1][lane] : 0);
+    if (lane == 0) {
+      compared.tops[0] = top_a;
+      compared.tops[1] = top_b;
+    }
+  }
+  __syncthreads();
+  cluster_meet();
+  // The row's, in every CTA's first warp.
+  Moments all = {};
+  u64 top_a = 0, top_b = 0;
+  if (warp == 0) {
+    Compared of = {{-kInfinity, 0.0f, 0.0f, 0.0f, 0.0f, 0}, {0, 0}};
+    if (lane < ranks) of = *of_rank(&compared, lane);
+    all = moments_of_lanes(of.moments);
+    top_a = warp_max(of.tops[0]);
+    top_b = warp_max(of.tops[1]);
+    if (lane == 0) {
+      s_beyond = all.beyond;
+      tops[0][0] = top_a;
+      tops[1][0] = top_b;
+    }
+  }
+  __syncthreads();
+  double kl = 0.0;
+  if (!s_beyond) {
+    const double mean_of = static_cast<double>(all.mean) / all.mass, rest_of = static_cast<double>(all.rest) / all.mass;
+    const double x = rest_of - mean_of;
+    // The same number; where x is large, the two would only cancel each other.
+    kl = fabs(x) < 0.5 ? rest_of + (log1p(x) - x) : mean_of + log1p(x);
+  } else {
+    const float most_a = value_of(static_cast<uint32_t>(tops[0][0] >> 32)), most_b = value_of(static_cast<uint32_t>(tops[1][0] >> 32));
+    const float b_there = E::one(b.data + place_of(tops[0][0]));
+    // Rows without a distribution (nothing but -inf, with NaN or with +inf); rows so far apart that e^(b - b*) overflows.
+    const bool none = !(fabsf(most_a) < kInfinity) || !(fabsf(most_b) < kInfinity), apart = !(most_b - b_there <= kNear);
+    sum = {};
+    if (!none) sum = far_moments(a, b, begin, end, most_a, apart ? most_b : b_there, apart);
+    cluster_meet();  // all have read the first ones
+    if (lane == 0) moments[warp] = sum;
+    __syncthreads();
+    cluster_meet();
+    if (rank == 0 && warp == 0) {
+      double mass_of = 0.0, mean_of = 0.0, rest_of = 0.0;
+      int infinite = 0;
+      for (int i = 0; i < ranks * kScoreWarps; ++i) {
+        const Moments of = *of_rank(&moments[i % kScoreWarps], i / kScoreWarps);
+        mass_of += of.mass;
+        mean_of += of.mean;
+        rest_of += of.rest;
+        infinite |= of.beyond;
+      }
       if (none) {
         kl = __longlong_as_double(0x7fffffffffffffffll);
       } else if (infinite) {
         kl = kInfinity;
-      } else if (far) {
-        kl = mean / mass + log(rest / mass);
+      } else if (apart) {
+        kl = mean_of / mass_of + log(rest_of / mass_of);
       } else {
-        const double remainder = rest / mass, x = remainder - mean / mass;
-        // The same number; where x is large, remainder and x would only cancel each other.
-        kl = fabs(x) < 0.5 ? remainder + (log1p(x) - x) : mean / mass + log1p(x);
+        const double remainder = rest_of / mass_of, x = remainder - mean_of / mass_of;
+        kl = fabs(x) < 0.5 ? remainder + (log1p(x) - x) : mean_of / mass_of + log1p(x);
       }
-      divergence[r] = static_cast<float>(kl < 0.0 ? 0.0 : kl);
-      agreement[r] = place_of(s_top[0]) == place_of(s_top[1]);
     }
+  }
+  if (rank == 0 && tid == 0) {
+    divergence[r] = static_cast<float>(kl < 0.0 ? 0.0 : kl);
+    agreement[r] = place_of(top_a) == place_of(top_b);
   }
   cluster_meet();  // the others' shared memory has been read
 }
 
 // ---- host ------------------------------------------------------------------------------------------
-constexpr int kMaxColumns = 1 << 21;  // elements that a thread may have to keep, 32 times over, fit shared memory
+constexpr int kMaxColumns = 1 << 21;
 
 static int element_bytes(int type) { return type == CFM_TYPE_F32 ? 4 : 2; }
 
@@ -661,11 +1019,21 @@ static int check_rows(const cfm_rows* rows, int most_columns) {
   return 0;
 }
 
-// CTAs that share a row.
+template <typename K>
+static int allow(K kernel, size_t shared) {
+  cudaError_t code = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(shared));
+  if (code == cudaSuccess) code = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+  return static_cast<int>(code);
+}
+
+// CTAs that share a row: until the call has 256, more than one for most SMs, or a thread has one piece.  What a CTA does after its
+// sums (5 to 8 us with top alternatives, all latency) grows with their number.  Log probabilities of 151936 BF16 logits,
+// us of 1, 2, 4, 8 and 16 CTAs per row: one row 14.5, 10.0, 7.3, 4.7, 4.2; 128 rows 15.1, 13.9, 15.1, 17.3; 512 rows 38.6, 38.3,
+// 48, 54, with 20 alternatives 63, 74, 102, 114.
 static int row_ranks(int rows, int columns, int type) {
   const int pieces = columns / (16 / element_bytes(type)) + 1;
   int ranks = 1;
-  while (ranks < kMaxCluster && static_cast<int64_t>(rows) * ranks < 592 && pieces > ranks * kScoreThreads) ranks *= 2;
+  while (ranks < kMaxCluster && static_cast<int64_t>(rows) * ranks < 256 && pieces > ranks * kScoreThreads) ranks *= 2;
   return ranks;
 }
 
@@ -687,17 +1055,9 @@ static int route(const cfm_rows* x, int K, int renormalize, void* ids, int ids64
 template <typename T>
 static int token_logprobs(const cfm_rows* x, const void* tokens, int tokens64, int n, float* logprobs, float* entropy,
                           int32_t* top_ids, float* top_logprobs, cudaStream_t stream) {
-  constexpr int W = Element<T>::kWidth;
   const int ranks = row_ranks(x->rows, x->columns, x->type);
-  // Pieces of a CTA, and elements of a thread, at most.
-  const int pieces = ((x->columns + W - 1) / W + 1 + ranks - 1) / ranks;
-  const size_t shared = sizeof(u64) * n * W * ((pieces + kScoreThreads - 1) / kScoreThreads);
-  if (shared > 40 * 1024) {
-    const cudaError_t code = cudaFuncSetAttribute(k_token_logprobs<T>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                                  static_cast<int>(shared));
-    if (code != cudaSuccess) return static_cast<int>(code);
-  }
-  launch_clusters(k_token_logprobs<T>, dim3(x->rows * ranks), dim3(kScoreThreads), shared, ranks, stream, x->data,
+  if (const int code = allow(k_token_logprobs<T>, kRingBytes)) return code;
+  launch_clusters(k_token_logprobs<T>, dim3(x->rows * ranks), dim3(kScoreThreads), kRingBytes, ranks, stream, x->data,
                   x->stride, x->columns, tokens, tokens64, n, logprobs, entropy, top_ids, top_logprobs);
   return launched();
 }
@@ -706,7 +1066,8 @@ template <typename T>
 static int compare_logits(const cfm_rows* a, const cfm_rows* b, float* divergence, uint8_t* agreement,
                           cudaStream_t stream) {
   const int ranks = row_ranks(a->rows, a->columns, a->type);
-  launch_clusters(k_compare_logits<T>, dim3(a->rows * ranks), dim3(kScoreThreads), 0, ranks, stream, a->data,
+  if (const int code = allow(k_compare_logits<T>, kCompareRing)) return code;
+  launch_clusters(k_compare_logits<T>, dim3(a->rows * ranks), dim3(kScoreThreads), kCompareRing, ranks, stream, a->data,
                   a->stride, b->data, b->stride, a->columns, divergence, agreement);
   return launched();
 }
