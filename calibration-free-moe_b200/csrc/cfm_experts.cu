@@ -489,12 +489,6 @@ int64_t lay_out(const cfm_experts* x, int64_t capacity, void* base, Scratch* s) 
   return at;
 }
 
-template <typename K>
-int allow_shared(K kernel, size_t bytes) {
-  if (bytes <= 48 * 1024) return 0;
-  return static_cast<int>(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(bytes)));
-}
-
 int run_few(const Experts& L, const Scratch& s, const Routes& routes, const __nv_bfloat16* hidden, int busy,
             __nv_bfloat16* out, cudaStream_t stream) {
   const int64_t items = static_cast<int64_t>(busy) * (L.I / 8);
@@ -539,8 +533,8 @@ int run_tensor(const Experts& L, const Scratch& s, const __nv_bfloat16* hidden, 
   CUtensorMap up, down;
   int code = make_map(&up, L.gate_up, static_cast<int64_t>(L.E) * 2 * L.I, L.H);
   if (!code) code = make_map(&down, L.down, static_cast<int64_t>(L.E) * L.I, L.H);
-  if (!code) code = allow_shared(k_experts_tensor<TOKENS, false>, U::kShared);
-  if (!code) code = allow_shared(k_experts_tensor<TOKENS, true>, D::kShared);
+  if (!code) code = allow_everything<k_experts_tensor<TOKENS, false>>(false);
+  if (!code) code = allow_everything<k_experts_tensor<TOKENS, true>>(false);
   if (code) return code;
   const int64_t passes = std::min<int64_t>(L.E, pairs) + pairs / TOKENS;
   const auto ctas = [&](int tiles) { return dim3(static_cast<unsigned>(std::min<int64_t>(148, passes * tiles))); };

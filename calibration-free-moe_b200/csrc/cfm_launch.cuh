@@ -3,9 +3,31 @@
 
 #include <cuda_runtime.h>
 
+#include <atomic>
+#include <cstdint>
 #include <cstdlib>
 
 namespace cfm {
+
+// Lets a kernel have as much shared memory, and clusters of as many CTAs, as the device has.  Once per kernel and
+// device (of the first 64): the two calls take 1.5 us of a launch.
+template <auto KERNEL>
+static int allow_everything(bool large_clusters) {
+  static std::atomic<uint64_t> done{0};
+  int device = 0;
+  cudaError_t code = cudaGetDevice(&device);
+  const uint64_t bit = device < 64 ? 1ull << device : 0;
+  if (code != cudaSuccess || (done.load(std::memory_order_relaxed) & bit)) return static_cast<int>(code);
+  cudaFuncAttributes attributes;
+  int most = 0;
+  code = cudaFuncGetAttributes(&attributes, KERNEL);
+  if (code == cudaSuccess) code = cudaDeviceGetAttribute(&most, cudaDevAttrMaxSharedMemoryPerBlockOptin, device);
+  if (code == cudaSuccess)
+    code = cudaFuncSetAttribute(KERNEL, cudaFuncAttributeMaxDynamicSharedMemorySize, most - static_cast<int>(attributes.sharedSizeBytes));
+  if (code == cudaSuccess && large_clusters) code = cudaFuncSetAttribute(KERNEL, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+  if (code == cudaSuccess) done.fetch_or(bit, std::memory_order_relaxed);
+  return static_cast<int>(code);
+}
 
 // Launch with programmatic stream serialisation: the kernel may be scheduled while its
 // predecessor in the stream is finishing and waits for it at grid_dependency_wait().

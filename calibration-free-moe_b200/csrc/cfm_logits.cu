@@ -1019,13 +1019,6 @@ static int check_rows(const cfm_rows* rows, int most_columns) {
   return 0;
 }
 
-template <typename K>
-static int allow(K kernel, size_t shared) {
-  cudaError_t code = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(shared));
-  if (code == cudaSuccess) code = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
-  return static_cast<int>(code);
-}
-
 // CTAs that share a row: until the call has 256, more than one for most SMs, or a thread has one piece.  What a CTA does after its
 // sums (5 to 8 us with top alternatives, all latency) grows with their number.  Log probabilities of 151936 BF16 logits,
 // us of 1, 2, 4, 8 and 16 CTAs per row: one row 14.5, 10.0, 7.3, 4.7, 4.2; 128 rows 15.1, 13.9, 15.1, 17.3; 512 rows 38.6, 38.3,
@@ -1056,7 +1049,7 @@ template <typename T>
 static int token_logprobs(const cfm_rows* x, const void* tokens, int tokens64, int n, float* logprobs, float* entropy,
                           int32_t* top_ids, float* top_logprobs, cudaStream_t stream) {
   const int ranks = row_ranks(x->rows, x->columns, x->type);
-  if (const int code = allow(k_token_logprobs<T>, kRingBytes)) return code;
+  if (const int code = allow_everything<k_token_logprobs<T>>(true)) return code;
   launch_clusters(k_token_logprobs<T>, dim3(x->rows * ranks), dim3(kScoreThreads), kRingBytes, ranks, stream, x->data,
                   x->stride, x->columns, tokens, tokens64, n, logprobs, entropy, top_ids, top_logprobs);
   return launched();
@@ -1066,7 +1059,7 @@ template <typename T>
 static int compare_logits(const cfm_rows* a, const cfm_rows* b, float* divergence, uint8_t* agreement,
                           cudaStream_t stream) {
   const int ranks = row_ranks(a->rows, a->columns, a->type);
-  if (const int code = allow(k_compare_logits<T>, kCompareRing)) return code;
+  if (const int code = allow_everything<k_compare_logits<T>>(true)) return code;
   launch_clusters(k_compare_logits<T>, dim3(a->rows * ranks), dim3(kScoreThreads), kCompareRing, ranks, stream, a->data,
                   a->stride, b->data, b->stride, a->columns, divergence, agreement);
   return launched();

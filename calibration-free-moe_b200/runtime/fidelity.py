@@ -10,7 +10,7 @@ from typing import NamedTuple
 import torch
 from torch import Tensor
 
-from .rows import byref, check_rows, enqueue, rows_struct
+from .rows import byref, check_rows, enqueue
 
 MAX_VOCABULARY = 1 << 21
 MAX_TOP = 32
@@ -35,26 +35,28 @@ def token_logprobs(logits: Tensor, tokens: Tensor, top: int = 0) -> TokenScores:
     +inf, or all of whose tokens are banned, has NaN for all its numbers.  Enqueued on the
     current stream; no gradients.
     """
-    check_rows(logits, "Logits", MAX_VOCABULARY)
+    struct, rows = check_rows(logits, "Logits", MAX_VOCABULARY)
+    index, wide = logits.get_device(), tokens.dtype is torch.int64
     if (
-        tokens.shape != logits.shape[:1]
-        or tokens.dtype not in (torch.int32, torch.int64)
-        or tokens.device != logits.device
+        tokens.shape != (rows,)
+        or not (wide or tokens.dtype is torch.int32)
+        or not tokens.is_cuda
+        or tokens.get_device() != index
         or not tokens.is_contiguous()
     ):
         raise ValueError("Tokens must be contiguous int32 or int64 [rows] on the logits' device")
-    if not 0 <= top <= min(MAX_TOP, logits.shape[1]):
+    if not 0 <= top <= MAX_TOP or top > struct.columns:
         raise ValueError(f"top must be from 0 to {MAX_TOP} and at most the vocabulary's size")
-    rows, device = logits.shape[0], logits.device
-    logprobs = torch.empty(rows, device=device, dtype=torch.float32)
-    entropy = torch.empty(rows, device=device, dtype=torch.float32)
-    top_ids = top_logprobs = None
-    if top:
-        top_ids = torch.empty((rows, top), device=device, dtype=torch.int32)
-        top_logprobs = torch.empty((rows, top), device=device, dtype=torch.float32)
-    enqueue("cfm_token_logprobs", device, byref(rows_struct(logits)), tokens.data_ptr(),
-            tokens.dtype == torch.int64, top, logprobs.data_ptr(), entropy.data_ptr(),
-            top_ids.data_ptr() if top else None, top_logprobs.data_ptr() if top else None)
+    logprobs = logits.new_empty(rows, dtype=torch.float32)
+    entropy = logits.new_empty(rows, dtype=torch.float32)
+    if not top:
+        enqueue("cfm_token_logprobs", index, byref(struct), tokens.data_ptr(), wide, 0,
+                logprobs.data_ptr(), entropy.data_ptr(), None, None)
+        return TokenScores(logprobs, entropy, None, None)
+    top_ids = logits.new_empty((rows, top), dtype=torch.int32)
+    top_logprobs = logits.new_empty((rows, top), dtype=torch.float32)
+    enqueue("cfm_token_logprobs", index, byref(struct), tokens.data_ptr(), wide, top,
+            logprobs.data_ptr(), entropy.data_ptr(), top_ids.data_ptr(), top_logprobs.data_ptr())
     return TokenScores(logprobs, entropy, top_ids, top_logprobs)
 
 
@@ -69,16 +71,16 @@ def compare_logits(reference: Tensor, logits: Tensor) -> tuple[Tensor, Tensor]:
     where a row has NaN or +inf or is banned altogether.  Enqueued on the current stream; no
     gradients.
     """
-    check_rows(reference, "Reference logits", MAX_VOCABULARY)
-    check_rows(logits, "Logits", MAX_VOCABULARY)
+    one, _ = check_rows(reference, "Reference logits", MAX_VOCABULARY)
+    other, rows = check_rows(logits, "Logits", MAX_VOCABULARY)
+    index = logits.get_device()
     if (
-        reference.shape != logits.shape
-        or reference.dtype != logits.dtype
-        or reference.device != logits.device
+        one.rows != rows or one.columns != other.columns or one.type != other.type
+        or reference.get_device() != index
     ):
         raise ValueError("Both rows of logits must have one shape, type and device")
-    divergence = torch.empty(logits.shape[0], device=logits.device, dtype=torch.float32)
-    agreement = torch.empty(logits.shape[0], device=logits.device, dtype=torch.bool)
-    enqueue("cfm_compare_logits", logits.device, byref(rows_struct(reference)),
-            byref(rows_struct(logits)), divergence.data_ptr(), agreement.data_ptr())
+    divergence = logits.new_empty(rows, dtype=torch.float32)
+    agreement = logits.new_empty(rows, dtype=torch.bool)
+    enqueue("cfm_compare_logits", index, byref(one), byref(other), divergence.data_ptr(),
+            agreement.data_ptr())
     return divergence, agreement

@@ -8,7 +8,7 @@ from __future__ import annotations
 import torch
 from torch import Tensor
 
-from .rows import byref, check_rows, enqueue, rows_struct
+from .rows import byref, check_rows, enqueue
 
 MAX_EXPERTS = 1024
 MAX_TOP_K = 32
@@ -31,17 +31,16 @@ def route_tokens(
     or of nothing but -inf has weights of NaN.  What a reader takes as `topk_ids` and
     `topk_weights`.  Enqueued on the current stream; no gradients.
     """
-    check_rows(logits, "Router logits", MAX_EXPERTS)
-    if not 1 <= top_k <= min(MAX_TOP_K, logits.shape[1]):
+    struct, rows = check_rows(logits, "Router logits", MAX_EXPERTS)
+    if not 1 <= top_k <= MAX_TOP_K or top_k > struct.columns:
         raise ValueError(f"top_k must be from 1 to {MAX_TOP_K} and at most the number of experts")
     if weights_dtype not in (torch.float32, torch.bfloat16):
         raise ValueError("Router weights are FP32 or BF16")
     if ids_dtype not in (torch.int32, torch.int64):
         raise ValueError("Expert ids are int32 or int64")
-    shape = (logits.shape[0], top_k)
-    weights = torch.empty(shape, device=logits.device, dtype=weights_dtype)
-    ids = torch.empty(shape, device=logits.device, dtype=ids_dtype)
-    enqueue("cfm_route_tokens", logits.device, byref(rows_struct(logits)), top_k, renormalize,
-            ids.data_ptr(), ids_dtype == torch.int64, weights.data_ptr(),
-            weights_dtype == torch.bfloat16)
+    weights = logits.new_empty((rows, top_k), dtype=weights_dtype)
+    ids = logits.new_empty((rows, top_k), dtype=ids_dtype)
+    enqueue("cfm_route_tokens", logits.get_device(), byref(struct), top_k, renormalize,
+            ids.data_ptr(), ids_dtype is torch.int64, weights.data_ptr(),
+            weights_dtype is torch.bfloat16)
     return weights, ids

@@ -3,6 +3,7 @@
 from __future__ import annotations
 
 import ctypes
+from functools import cache
 
 import torch
 from torch import Tensor
@@ -12,34 +13,36 @@ from .. import _native
 TYPE_CODES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
 
 
-def check_rows(logits: Tensor, what: str, most_columns: int) -> None:
-    """Raise ValueError unless `logits` is a CUDA matrix of contiguous BF16, FP16 or FP32 rows."""
-    if (
-        logits.ndim != 2
-        or logits.dtype not in TYPE_CODES
-        or not logits.is_cuda
-        or not 1 <= logits.shape[1] <= most_columns
-        or logits.shape[0] > 2**28
-    ):
-        raise ValueError(
-            f"{what} must be a CUDA tensor [rows, columns] of BF16, FP16 or FP32 with 1 to "
-            f"{most_columns} columns")
-    if (logits.shape[1] > 1 and logits.stride(1) != 1) or (
-            logits.shape[0] > 1 and logits.stride(0) < logits.shape[1]):
+def check_rows(logits: Tensor, what: str, most_columns: int) -> tuple[_native.Rows, int]:
+    """The rows as a structure, and their number; ValueError unless `logits` is a CUDA matrix of
+    contiguous BF16, FP16 or FP32 rows."""
+    shape = logits.shape
+    code = TYPE_CODES.get(logits.dtype)
+    if code is None or len(shape) != 2 or not logits.is_cuda:
+        raise ValueError(f"{what} must be a CUDA tensor [rows, columns] of BF16, FP16 or FP32")
+    rows, columns = shape
+    if not 1 <= columns <= most_columns or rows > 2**26:
+        raise ValueError(f"{what} must have 1 to {most_columns} columns and at most 2^26 rows")
+    step, one = logits.stride()
+    if (one != 1 and columns > 1) or (step < columns and rows > 1):
         raise ValueError(f"{what} must have contiguous rows that do not overlap")
     if logits.requires_grad and torch.is_grad_enabled():
         raise ValueError(f"{what} requires grad: this operator has no backward pass")
+    return _native.Rows(logits.data_ptr(), step, rows, columns, code), rows
 
 
-def rows_struct(logits: Tensor) -> _native.Rows:
-    return _native.Rows(logits.data_ptr(), logits.stride(0), logits.shape[0], logits.shape[1],
-                        TYPE_CODES[logits.dtype])
+byref = ctypes.byref
 
 
-def enqueue(name: str, device: torch.device, *arguments: object) -> None:
-    """Call an entry point of the library with the current stream of `device` at the end."""
-    function = getattr(_native.load(), name)
-    index = device.index
+@cache
+def entry_point(name: str):
+    """A function of the library, which is loaded on first use."""
+    return getattr(_native.load(), name)
+
+
+def enqueue(name: str, index: int, *arguments: object) -> None:
+    """Call an entry point with the current stream of device `index` as its last argument."""
+    function = entry_point(name)
     if torch.cuda.current_device() == index:
         code = function(*arguments, torch._C._cuda_getCurrentRawStream(index))
     else:
@@ -47,7 +50,3 @@ def enqueue(name: str, device: torch.device, *arguments: object) -> None:
             code = function(*arguments, torch._C._cuda_getCurrentRawStream(index))
     if code:
         _native.check(code, name)
-
-
-def byref(rows: _native.Rows):
-    return ctypes.byref(rows)
