@@ -518,13 +518,12 @@ int make_map(CUtensorMap* map, const void* data, int64_t rows, int64_t columns) 
   return code == CUDA_SUCCESS ? 0 : static_cast<int>(cudaErrorInvalidValue);
 }
 
-// Pairs of a pass, for `busy` experts.  A second pass over an expert reads its weights again, from L2; a stage with room for more
-// tokens leaves fewer stages in the ring.  Passes of 16, 32, 64, 128 (and 192), us of a call: 64 tokens of the
-// 128-expert layer (4 per expert) 200, 195, 196, 205; 256 of 256 experts with a skewed router (8) 192, 168, 168, 169;
-// 1000 of 64 experts (125) 828, 452, 299, 234, 216.
-int pass_pairs(int64_t pairs, int64_t busy) {
-  return pairs <= 12 * busy ? 32 : pairs <= 32 * busy ? 64 : pairs <= 80 * busy ? 128 : 192;
-}
+// Pairs of a pass, for `busy` experts.  A second pass over an expert reads its weights again, from L2; a stage with room for
+// more tokens leaves fewer stages in the ring.  Passes of 16, 32, 64 and 128, us of a call: 64 tokens of the
+// 128-expert layer (4 per expert) 200, 195, 196, 205; 256 of 256 experts with a skewed router (8) 192, 168, 168, 169.  Of 128, 144,
+// 160 and 192: 400 of 64 experts of width 768 (50) 145, 141, 150, 151; 1000 of 64 experts of width 1024 (125) 275, 267, 261, 263;
+// 1000 of 32 experts of hidden 1024 (250) 129, 121, 131, 142.
+int pass_pairs(int64_t pairs, int64_t busy) { return pairs <= 12 * busy ? 32 : pairs <= 40 * busy ? 64 : 144; }
 
 template <int TOKENS>
 int run_tensor(const Experts& L, const Scratch& s, const __nv_bfloat16* hidden, int64_t pairs, cudaStream_t stream) {
@@ -578,10 +577,9 @@ int cfm_experts_forward(const cfm_experts* layer, void* workspace, int32_t capac
   if (pairs <= kFewPairs) return run_few(L, s, routes, hidden, busy, out, st);
   const int pass = pass_pairs(pairs, busy);
   launch_dependent(k_group_pairs, dim3(1), dim3(kGroupThreads), sizeof(int) * L.E, st, routes, L.E, L.K, pass, s);
-  const int code = pass == 32    ? run_tensor<32>(L, s, hidden, pairs, st)
-                   : pass == 64  ? run_tensor<64>(L, s, hidden, pairs, st)
-                   : pass == 128 ? run_tensor<128>(L, s, hidden, pairs, st)
-                                 : run_tensor<192>(L, s, hidden, pairs, st);
+  const int code = pass == 32   ? run_tensor<32>(L, s, hidden, pairs, st)
+                   : pass == 64 ? run_tensor<64>(L, s, hidden, pairs, st)
+                                : run_tensor<144>(L, s, hidden, pairs, st);
   if (code) return code;
   launch_dependent(k_experts_mix, dim3(call->tokens, (L.H + 8 * kMixThreads - 1) / (8 * kMixThreads)), dim3(kMixThreads), 0,
                    st, L, s, routes, out);
