@@ -564,6 +564,8 @@ int cfm_experts_forward(const cfm_experts* layer, void* workspace, int32_t capac
   if (!call || !workspace || !layer->gate_up || !layer->down || !call->hidden || !call->ids || !call->weights || !call->out)
     return CFM_E_NULL;
   if (call->tokens < 1 || call->tokens > capacity) return CFM_E_CAPACITY;
+  for (const void* p : {layer->gate_up, layer->down, call->hidden, static_cast<const void*>(call->out), static_cast<const void*>(workspace)})
+    if (reinterpret_cast<uintptr_t>(p) % 16) return CFM_E_SHAPE;
   Scratch s;
   lay_out(layer, capacity, workspace, &s);
   const Experts L = {layer->hidden, layer->width, layer->experts, layer->top_k, layer->activation,

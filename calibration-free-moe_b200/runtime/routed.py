@@ -3,7 +3,8 @@
 `ProgressiveReader` reads the channels that it keeps; `RoutedExperts` reads all of them, from the
 same tensors and with the same call, for one token to thousands.  It is the stock side of
 `ProgressiveExperts` without an engine (`RoutedExperts.rows`), which `experts.dense_routed_experts` is in
-torch operations, and the run that a sparse one is held against.
+torch operations, and the run that a sparse one is held against.  `ops.register_reader` takes one as it
+takes a reader.
 """
 
 from __future__ import annotations

@@ -51,6 +51,8 @@ from ..reader.bank import subspace_bank
 from ..reader.budget import compile_budget
 from ..reader.progressive import ProgressiveReader, ReaderWorkspace, channel_major_down
 from .experts import PhaseContext, ProgressiveExperts
+from .fidelity import compare_logits, token_logprobs
+from .routing import route_tokens
 
 
 def decode_rows(metadata: Any, tokens: int) -> int:
@@ -94,18 +96,29 @@ def dense_block(gate_up: Tensor, down: Tensor, x: Tensor, weights: Tensor, ids: 
     return out
 
 
+ROUTERS = ("torch", "library")
+
+
 class BoundBlock:
     """What replaces `forward` of one sparse-MoE block."""
 
     def __init__(self, block: torch.nn.Module, experts: ProgressiveExperts, top_k: int,
-                 renormalize: bool) -> None:
+                 renormalize: bool, router: str = "torch") -> None:
+        if router not in ROUTERS:
+            raise ValueError(f"router must be one of {ROUTERS}")
         self.block, self.experts = block, experts
-        self.top_k, self.renormalize = top_k, renormalize
+        self.top_k, self.renormalize, self.router = top_k, renormalize, router
         self.stock_forward = block.forward
         self.sparse_rows = 0
         self.verify = False
         self.enabled = True   # False: decode rows take the stock block too (the comparison run)
         self.timed: list[tuple[torch.cuda.Event, torch.cuda.Event]] | None = None
+
+    def route(self, logits: Tensor) -> tuple[Tensor, Tensor]:
+        """Router weights and ids of the decode rows, in torch operations or in one launch."""
+        if self.router == "library":
+            return route_tokens(logits, self.top_k, renormalize=self.renormalize)
+        return route(logits, self.top_k, self.renormalize)
 
     def block_microseconds(self) -> float:
         """Mean device time of this block over the decode steps recorded since `timed = []`."""
@@ -152,7 +165,7 @@ class BoundBlock:
             start.record()
         if self.enabled:
             logits, _ = self.block.gate(x)
-            weights, ids = route(logits, self.top_k, self.renormalize)
+            weights, ids = self.route(logits)
             self.sparse_rows += rows
             context = PhaseContext(num_decode_tokens=rows)
             out = self.experts.forward_modular(x, weights, ids, context).view(hidden_states.shape)
@@ -175,11 +188,14 @@ def moe_blocks(model: torch.nn.Module) -> list[tuple[str, torch.nn.Module]]:
 
 @torch.no_grad()
 def bind(model: torch.nn.Module, *, retention: float, screen_keep: float, rank: int,
-         max_tokens: int, selection_score: str = "point") -> list[BoundBlock]:
+         max_tokens: int, selection_score: str = "point",
+         router: str = "torch") -> list[BoundBlock]:
     """Build one reader per sparse-MoE block of `model` and route its decode rows through it.
 
     Returns the bound blocks (`unbind` restores the stock forwards).  One workspace
     serves all layers, as in the reference's hook (`runtime/experts.py:1210-1243`).
+    `router="library"` takes the router outputs from `route_tokens`, one launch per block; equal
+    logits then go to the lowest expert, which `torch.topk` does not say.
     """
     bound: list[BoundBlock] = []
     workspace = None
@@ -211,7 +227,8 @@ def bind(model: torch.nn.Module, *, retention: float, screen_keep: float, rank: 
         def stock_rows(x: Tensor, _weights: Tensor, _ids: Tensor, forward=stock) -> Tensor:
             return forward(x)
 
-        replacement = BoundBlock(block, ProgressiveExperts(reader, stock_rows), top_k, renormalize)
+        replacement = BoundBlock(block, ProgressiveExperts(reader, stock_rows), top_k, renormalize,
+                                 router)
         replacement.verify = index == 0  # one block stands for the backend's weight layout
         block.forward = replacement
         bound.append(replacement)
@@ -252,10 +269,14 @@ MODEL_CONFIG = {
 
 class LogitsTap:
     """Wraps `model.compute_logits`: keeps every step's logits, or scores them against kept
-    ones and returns the kept ones, so that the sampled tokens repeat the first run's."""
+    ones and returns the kept ones, so that the sampled tokens repeat the first run's.  With
+    `library` the scores come from the library's kernels, and there are two more: each row's entropy
+    in the first run, and the log probability that the second gives to the token of the first."""
 
-    def __init__(self, model: torch.nn.Module) -> None:
-        self.model, self.stock = model, model.compute_logits
+    def __init__(self, model: torch.nn.Module, library: bool = False) -> None:
+        self.model, self.stock, self.library = model, model.compute_logits, library
+        self.entropy: list[Tensor] = []
+        self.logprobs: list[Tensor] = []
         self.kept: list[Tensor] = []
         self.kl: list[Tensor] = []
         self.agree: list[Tensor] = []
@@ -274,7 +295,13 @@ class LogitsTap:
             self.kept.append(logits.detach().clone())
             return logits
         reference = self.kept[self.step]
-        divergence, same = kl_and_top1(reference, logits)
+        if self.library:
+            divergence, same = compare_logits(reference, logits)
+            tokens = reference.argmax(dim=-1)
+            self.entropy.append(token_logprobs(reference, tokens).entropy)
+            self.logprobs.append(token_logprobs(logits, tokens).logprobs)
+        else:
+            divergence, same = kl_and_top1(reference, logits)
         self.kl.append(divergence)
         self.agree.append(same)
         self.step += 1
@@ -287,8 +314,12 @@ class LogitsTap:
 def decode_study(*, layers: int = 48, batch: int = 32, prompt_tokens: int = 4096,
                  decode_tokens: int = 256, retention: float = 0.123046875,
                  screen_keep: float = 0.625, rank: int = 64, seed: int = 0,
-                 memory_fraction: float = 0.55) -> dict:
-    """Stock and sparse greedy decode of a random-weight Qwen3-30B-A3B-shaped model in vLLM."""
+                 memory_fraction: float = 0.55, library: bool = False) -> dict:
+    """Stock and sparse greedy decode of a random-weight Qwen3-30B-A3B-shaped model in vLLM.
+
+    With `library` the router outputs of the sparse run and the scores of both come from the library's
+    kernels (`runtime/routing.py`, `runtime/fidelity.py`), and the report has two more scores.
+    """
     os.environ.setdefault("VLLM_ENABLE_V1_MULTIPROCESSING", "0")  # the model lives in this process
     from vllm import LLM, SamplingParams
 
@@ -316,7 +347,7 @@ def decode_study(*, layers: int = 48, batch: int = 32, prompt_tokens: int = 4096
         return count
 
     parameters = llm.apply_model(initialise)[0]
-    taps = llm.apply_model(LogitsTap)
+    taps = llm.apply_model(lambda model: LogitsTap(model, library))
     tap = taps[0]
     generator = torch.Generator().manual_seed(seed)
     prompts = [
@@ -337,7 +368,8 @@ def decode_study(*, layers: int = 48, batch: int = 32, prompt_tokens: int = 4096
 
     started = time.perf_counter()
     bound = llm.apply_model(lambda model: bind(
-        model, retention=retention, screen_keep=screen_keep, rank=rank, max_tokens=batch))[0]
+        model, retention=retention, screen_keep=screen_keep, rank=rank, max_tokens=batch,
+        router="library" if library else "torch"))[0]
     bind_seconds = time.perf_counter() - started
 
     def arm(enabled: bool) -> None:
@@ -361,7 +393,12 @@ def decode_study(*, layers: int = 48, batch: int = 32, prompt_tokens: int = 4096
     divergence = torch.stack(tap.kl[1:]).float()  # step 0 is the prefill step (stock in both runs)
     agreement = torch.stack(tap.agree[1:]).float()
     reports = [replacement.experts.reader.report() for replacement in bound[:1]]
+    more = {}
+    if library:
+        more = {"stock_entropy_mean": float(torch.stack(tap.entropy[1:]).mean()),
+                "sparse_logprob_of_stock_token_mean": float(torch.stack(tap.logprobs[1:]).mean())}
     return {
+        **more,
         "model": f"Qwen3-30B-A3B-shaped, {layers} layers, random weights N(0, 0.02^2), "
                  f"{parameters / 1e9:.1f} B parameters",
         "engine": "vLLM 0.22 in process, eager, one prefill step then greedy decode",
@@ -388,8 +425,10 @@ if __name__ == "__main__":
     parser.add_argument("--decode-tokens", type=int, default=256)
     parser.add_argument("--memory-fraction", type=float, default=0.55,
                         help="share of the GPU's memory the engine may take (weights and KV cache)")
+    parser.add_argument("--library", action="store_true",
+                        help="router outputs and scores by the library's kernels")
     arguments = parser.parse_args()
-    print(json.dumps(decode_study(layers=arguments.layers, batch=arguments.batch,
+    print(json.dumps(decode_study(library=arguments.library, layers=arguments.layers, batch=arguments.batch,
                                   prompt_tokens=arguments.prompt_tokens,
                                   decode_tokens=arguments.decode_tokens,
                                   memory_fraction=arguments.memory_fraction)))

@@ -89,12 +89,13 @@ def test_router_ties_and_rows_without_a_distribution():
 def check_scores(x, tokens, top):
     got = token_logprobs(x, tokens, top)
     wide = x.double()
-    total = torch.logsumexp(wide, dim=-1)
-    log_p = wide - total[:, None]
-    log_p[~total.isfinite()] = math.nan  # no distribution
-    p = log_p.exp()
     largest = wide.amax(-1)
-    rest = 1.0 - (largest - total).exp()  # what the largest does not have
+    shifted = wide - largest[:, None]
+    log_z = shifted.exp().sum(-1).log()
+    log_p = shifted - log_z[:, None]
+    log_p[~largest.isfinite()] = math.nan  # no distribution
+    p = log_p.exp()
+    rest = 1.0 - (-log_z).exp()  # what the largest does not have
     ok = (tokens >= 0) & (tokens < x.shape[1])
     want = log_p.gather(1, tokens.clamp(0, x.shape[1] - 1).long()[:, None])[:, 0]
     assert got.logprobs[~ok].isnan().all()
@@ -105,11 +106,11 @@ def check_scores(x, tokens, top):
         assert (off <= allowed.nan_to_num(0.0, 0.0, 0.0)).all(), (off - allowed).max().item()
 
     # The difference to the largest, the logarithm's sum, the result.
-    allowed = SUM * rest + 4 * STEP * (want.abs() + (want + total - largest).abs())
+    allowed = SUM * rest + 4 * STEP * (want.abs() + (want + log_z).abs())
     near(got.logprobs[ok], want[ok], allowed[ok])
     entropy = -torch.where(log_p > -math.inf, p * log_p, 0.0).sum(-1)
     spread = torch.where(p > 0, p * (largest[:, None] - wide), 0.0).sum(-1)
-    entropy = torch.where(total.isfinite(), entropy, math.nan)
+    entropy = torch.where(largest.isfinite(), entropy, math.nan)
     near(got.entropy, entropy, SUM * (rest + 2 * spread) + 4 * STEP * entropy)
     if top:
         ids = ranked(x, top)
@@ -262,6 +263,40 @@ def test_divergence_of_rows_too_far_apart_for_one_shift():
     a[1, 3], b[1, 900] = 1.0, 300.0
     b[2, 10] = 61.0
     check_divergence(a, b)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_rows_beyond_32_bits_of_elements(dtype):
+    buffer = torch.empty(2**31 + 5000, device="cuda", dtype=dtype)
+    x, y = buffer[:5000 + 2**31].as_strided((3, 1000), (2**30, 1)), logits(3, 1000, dtype, 5)
+    x.copy_(logits(3, 1000, dtype, 4))
+    tokens = torch.tensor([0, 999, 5], device="cuda")
+    check_scores(x, tokens, 7)
+    check_divergence(x, y)
+    weights, ids = route_tokens(x, 6)
+    assert torch.equal(ids.long(), ranked(x, 6)) and torch.equal(weights, route_tokens(x.contiguous(), 6)[0])
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_huge_values(dtype):
+    """Values whose multiples of log2 e are not finite, and the largest of their type."""
+    most = torch.finfo(dtype).max
+    x = logits(6, 3000, dtype, 8)
+    x[0, 5], x[1, 7], x[2] = most, most / 2, -most
+    x[2, 11], x[3, 4], x[4, 100:200] = -most / 2, -most, most
+    tokens = torch.tensor([5, 7, 11, 4, 150, 0], device="cuda")
+    check_scores(x, tokens, 9)
+    check_divergence(x, x)
+    divergence, agreement = compare_logits(x, x)
+    assert not divergence.any() and agreement.all()
+
+
+@pytest.mark.parametrize("vocabulary,top", [(300000, 32), (1 << 21, 20)])
+def test_many_equal_rows_of_a_large_vocabulary(vocabulary, top):
+    """More elements as large as the threads' maxima than are sorted at a time."""
+    x = (torch.arange(vocabulary, device="cuda") % 7).bfloat16().expand(2, vocabulary).contiguous()
+    x[1] = torch.sort(logits(1, vocabulary, torch.bfloat16, 3)[0]).values
+    check_scores(x, torch.tensor([6, vocabulary - 1], device="cuda"), top)
 
 
 # -- calls -----------------------------------------------------------------------------------

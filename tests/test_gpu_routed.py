@@ -222,6 +222,64 @@ def test_stock_rows_of_the_engine_side_caller():
     assert run.rows(x[:0], weights[:0], ids[:0]).shape == (0, 256)
 
 
+def test_weights_beyond_32_bits_of_elements():
+    """The last expert of a layer whose gate and up rows are more than 2^31 elements."""
+    hidden, width, experts = 8192, 1024, 130
+    gate_up = torch.zeros((experts, 2 * width, hidden), device="cuda", dtype=torch.bfloat16)
+    down = torch.zeros((experts, width, hidden), device="cuda", dtype=torch.bfloat16)
+    assert gate_up[:-1].numel() > 2**31
+    for expert in (0, experts - 1):
+        for weight in (gate_up, down):
+            weight[expert].normal_(0.0, 0.02, generator=torch.Generator(device="cuda").manual_seed(expert))
+    small_gate_up, small_down = gate_up[[0, -1]], down[[0, -1]].transpose(1, 2)
+    for tokens in (2, 20):
+        x, ids, weights = batch(tokens, hidden, 2, 2)
+        want = RoutedExperts(small_gate_up, small_down, 2, tokens)(x, ids, weights)
+        got = RoutedExperts(gate_up, down.transpose(1, 2), 2, tokens)(x, ids * (experts - 1), weights)
+        assert torch.equal(got, want) and got.any()
+
+
+def test_as_an_opaque_operator():
+    from cfm_b200.runtime import ops
+
+    gate_up, down = layer(256, 48, 4)
+    x, ids, weights = batch(20, 256, 4, 2)
+    run = RoutedExperts(gate_up, down, 2, 20)
+    out = torch.empty_like(x)
+    torch.ops.cfm_b200.reader_forward(x, ids, weights, None, out, ops.register_reader(run))
+    assert torch.equal(out, run(x, ids, weights))
+
+
+def test_beside_the_reader_that_keeps_all_channels():
+    """A reader that keeps every channel computes the same layer, from the same tensors."""
+    from cfm_b200.reader.budget import compile_budget
+    from cfm_b200.reader.progressive import ProgressiveReader
+
+    gate_up, down = layer(256, 48, 4)
+    x, ids, weights = batch(12, 256, 4, 2)
+    plan = compile_budget(hidden_size=256, expert_width=48, top_k=2, retention=1.0, screen_keep=1.0)
+    reader = ProgressiveReader(gate_up, down, None, None, plan, 12, selection_score="point")
+    got, kept = RoutedExperts(gate_up, down, 2, 12)(x, ids, weights), reader(x, ids, weights)
+    # The reader rounds gate, up, their product twice and each expert's sum to BF16.
+    assert (got.float() - kept.float()).norm() < 0.02 * kept.float().norm()
+
+
+def test_two_calls_at_once_with_workspaces_of_their_own():
+    gate_up, down = layer(512, 96, 8)
+    runs = [RoutedExperts(gate_up, down, 2, 200) for _ in range(2)]
+    inputs = [batch(tokens, 512, 8, 2, seed) for tokens, seed in ((200, 3), (90, 4))]
+    want = [run(*given) for run, given in zip(runs, inputs)]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in runs]
+    for _ in range(10):
+        got = []
+        for stream, run, given in zip(streams, runs, inputs):
+            with torch.cuda.stream(stream):
+                got.append(run(*given))
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
 def test_a_decode_step_from_router_to_scores():
     """Router, layer, head and scores as one captured step, against the same in 64 bits."""
     hidden, experts, vocabulary = 512, 16, 5003
