@@ -312,8 +312,9 @@ __global__ void __launch_bounds__(32 * kRouteRows)
 constexpr int kScoreThreads = 256;
 constexpr int kScoreWarps = kScoreThreads / 32;
 constexpr int kScorePerSm = 4;
-constexpr int kScorePieces = 5;                 // of a thread that are added up together
-constexpr int kScoreRing = 2 * kScorePieces;    // that are on their way or kept
+constexpr int kScorePieces = 3;                 // of a thread that are added up together
+constexpr int kScoreChunks = 2;                 // of so many pieces that are on their way or kept
+constexpr int kScoreRing = kScoreChunks * kScorePieces;
 constexpr size_t kRingBytes = static_cast<size_t>(kScoreThreads) * kScoreRing * 16;
 constexpr int kFound = 512;
 constexpr int kChunksKnown = 64;                // whose largest values the second pass looks at
@@ -413,8 +414,8 @@ __global__ void __launch_bounds__(kScoreThreads, kScorePerSm)
     }
     copy_async_commit();
   };
-  bring_chunk(begin, 0);
-  bring_chunk(begin + kChunk, kScorePieces);
+#pragma unroll 1
+  for (int i = 0; i < kScoreChunks; ++i) bring_chunk(begin + i * kChunk, kScorePieces * i);
   int64_t token = -1;
   if (rank == 0 && tid == 0)
     token = tokens64 ? static_cast<const int64_t*>(tokens)[r] : static_cast<const int32_t*>(tokens)[r];
@@ -423,8 +424,8 @@ __global__ void __launch_bounds__(kScoreThreads, kScorePerSm)
   int best_chunk = begin;
   float m = -kInfinity, equal = 0.0f, others = 0.0f, weighted = 0.0f;
   int slot = 0, number = 0;
-  for (int first = begin; first < end; first += kChunk, slot = kScorePieces - slot, ++number) {
-    copy_async_wait<1>();
+  for (int first = begin; first < end; first += kChunk, ++number) {
+    copy_async_wait<kScoreChunks - 1>();
     uint4 v[kScorePieces];
     typename E::Top highest = E::lowest();
 #pragma unroll
@@ -433,8 +434,9 @@ __global__ void __launch_bounds__(kScoreThreads, kScorePerSm)
       E::fold(highest, v[j]);
     }
     const float top = E::value(highest);
-    if (!kept) bring_chunk(first + 2 * kChunk, slot);
+    if (!kept) bring_chunk(first + kScoreChunks * kChunk, slot);
     else copy_async_commit();
+    slot = slot + kScorePieces == kScoreRing ? 0 : slot + kScorePieces;
     if (!(top <= best) && best == best) {
       best = top;
       best_chunk = first;
@@ -615,9 +617,11 @@ __global__ void __launch_bounds__(kScoreThreads, kScorePerSm)
 //   E[psi] + (log1p(x) - x),
 // where nothing of first order in t is left to cancel: rows that hardly differ keep their digits in FP32.
 // A shift is changed by D without loss: psi(t + D) = e^-D psi(t) + psi(D) - (e^-D - 1) t.
-constexpr int kComparePieces = 3;  // of a thread and row that are looked at together
+constexpr int kComparePieces = 2;  // of a thread and row that are looked at together
+constexpr int kCompareChunks = 2;  // that are on their way or looked at
 constexpr int kCompareChunk = kComparePieces * kScoreThreads;
-constexpr size_t kCompareRing = 4ull * kComparePieces * kScoreThreads * 16;  // two chunks of two rows
+constexpr size_t kCompareRing = 2ull * kCompareChunks * kComparePieces * kScoreThreads * 16;  // of two rows
+constexpr float kSlack = 2.0f;     // by which an a may be above its exponential's shift
 constexpr float kNear = 60.0f;     // |t| of the single pass; beyond, and where a row has -inf alone, NaN or +inf, there is another
 
 // psi(t) / t^2 for |t| up to 1/2: the series to t^6, whose last term the Chebyshev polynomial of degree six turns into
@@ -797,15 +801,15 @@ __global__ void __launch_bounds__(kScoreThreads, kScorePerSm)
     }
     copy_async_commit();
   };
-  bring_chunk(begin, 0);
-  bring_chunk(begin + kCompareChunk, 2 * kComparePieces);
+#pragma unroll 1
+  for (int i = 0; i < kCompareChunks; ++i) bring_chunk(begin + i * kCompareChunk, 2 * kComparePieces * i);
 
   float best_a = -kInfinity, best_b = -kInfinity;  // of the thread, NaN above all, and the first chunks that have them
   int chunk_a = begin, chunk_b = begin;
   Moments sum = {-kInfinity, 0.0f, 0.0f, 0.0f, 0.0f, 0};
   int slot = 0;
-  for (int first = begin; first < end; first += kCompareChunk, slot = 2 * kComparePieces - slot) {
-    copy_async_wait<1>();
+  for (int first = begin; first < end; first += kCompareChunk) {
+    copy_async_wait<kCompareChunks - 1>();
     typename E::Top high_a = E::lowest(), high_b = E::lowest();
 #pragma unroll
     for (int j = 0; j < kComparePieces; ++j) {
@@ -824,7 +828,7 @@ __global__ void __launch_bounds__(kScoreThreads, kScorePerSm)
     const float chunk = warp_max_nan(top_a);
     // Too large to be scaled, or NaN.
     if ((!(fabsf(chunk) <= kModerate) && chunk != -kInfinity) || top_b != top_b) sum.beyond = 1;
-    if (chunk > sum.m && chunk <= kModerate) {  // new shifts, the same in the whole warp: of its largest a
+    if (chunk > sum.m + kSlack && chunk <= kModerate) {  // new shifts, the same in the whole warp: of its largest a
       float d = 0.0f;
       if (top_a == chunk) {
 #pragma unroll 1
@@ -897,12 +901,21 @@ __global__ void __launch_bounds__(kScoreThreads, kScorePerSm)
       pair_split(rests, s0, s1);
       sum.rest = __fmaf_rn(s0 + s1, back, sum.rest);
     }
-    bring_chunk(first + 2 * kCompareChunk, slot);
+    bring_chunk(first + kCompareChunks * kCompareChunk, slot);
+    slot += 2 * kComparePieces;
+    if (slot == 2 * kComparePieces * kCompareChunks) slot = 0;
   }
   // The warps', the CTA's.
   const float high_a = warp_max_nan(best_a), high_b = warp_max_nan(best_b);
   {
-    const Moments all = moments_of_lanes(sum);
+    Moments all = sum;  // the shifts are the warp's
+#pragma unroll
+    for (int w = 16; w; w >>= 1) {
+      all.mass += __shfl_xor_sync(kFull, all.mass, w);
+      all.mean += __shfl_xor_sync(kFull, all.mean, w);
+      all.rest += __shfl_xor_sync(kFull, all.rest, w);
+      all.beyond |= __shfl_xor_sync(kFull, all.beyond, w);
+    }
     if (lane == 0) {
       moments[warp] = all;
       highs[0][warp] = high_a;
