@@ -91,7 +91,8 @@ __device__ __forceinline__ void mma_bf16(float (&c)[4], uint32_t a0, uint32_t a1
 // ---- group: one CTA --------------------------------------------------------------------------------
 // All latency (9 us of a call of 64 tokens when every pair was looked at twice and three sums were scanned): a
 // thread keeps its pairs' experts and their places among the expert's pairs, which one pass of atomics gives,
-// and the two sums are scanned as one number.  The order of an expert's pairs is as it comes.
+// and the two sums are scanned as one number.  The order of an expert's pairs is as it comes.  The list is put in order in shared
+// memory: 8000 pairs stored one by one took this CTA 9 of its 16 us.
 constexpr int kGroupThreads = 1024;
 constexpr int kGroupKept = 8;  // pairs of a thread that stay in registers; of larger calls the rest is looked at twice
 constexpr int64_t kMostPairs = 1 << 24;
@@ -100,7 +101,8 @@ constexpr int64_t kMostPairs = 1 << 24;
 __global__ void __launch_bounds__(kGroupThreads) k_group_pairs(Routes routes, int E, int K, int tokens, Scratch s) {
   extern __shared__ int group_shared[];
   __shared__ uint64_t warps[32];
-  int* count = group_shared;  // [E], then the first place of every expert
+  int* list = group_shared;                                    // [kGroupKept * kGroupThreads] pairs by expert
+  int* count = group_shared + kGroupKept * kGroupThreads;     // [E], then the first place of every expert
   const int tid = threadIdx.x, lane = tid & 31, pairs = routes.tokens * K;
   for (int e = tid; e < E; e += kGroupThreads) count[e] = 0;
   __syncthreads();
@@ -155,14 +157,28 @@ __global__ void __launch_bounds__(kGroupThreads) k_group_pairs(Routes routes, in
   }
   if (tid == 0) s.counts[0] = static_cast<int>(warps[31] >> kPassBits);
   __syncthreads();
+  const bool fits = pairs <= kGroupKept * kGroupThreads;
 #pragma unroll
   for (int j = 0; j < kGroupKept; ++j) {
     if (expert[j] < 0) continue;
     const int p = tid + j * kGroupThreads, at = count[expert[j]] + rank[j];
-    s.pairs[at] = p;
-    s.tokens[at] = p / K;
+    if (fits) {
+      list[at] = p;
+    } else {
+      s.pairs[at] = p;
+      s.tokens[at] = p / K;
+    }
   }
-  if (pairs <= kGroupKept * kGroupThreads) return;
+  if (fits) {
+    __syncthreads();
+    const int grouped = static_cast<int>(warps[31] & ((1u << kPassBits) - 1));
+    for (int at = tid; at < grouped; at += kGroupThreads) {
+      const int p = list[at];
+      s.pairs[at] = p;
+      s.tokens[at] = p / K;
+    }
+    return;
+  }
   // The other pairs come behind those.
   __syncthreads();
 #pragma unroll
@@ -426,33 +442,44 @@ __global__ void __launch_bounds__(kFewDownThreads, 2)
 #include "cfm_experts_tc.cuh"
 
 // ---- mix -------------------------------------------------------------------------------------------
-constexpr int kMixThreads = 128;
+constexpr int kMixThreads = 256;
+constexpr int kMixAhead = 8;  // slots whose sums are on their way
 
-// grid (T, H / 1024 and the rest): eight columns of a token per thread.
+// grid (T, H / 1024 and the rest): four columns of a token per thread.  The routes are asked for before the sums are there,
+// and the sums of several slots at a time (one slot after another: 9.6 us for 64 tokens).
 __global__ void __launch_bounds__(kMixThreads) k_experts_mix(Experts L, Scratch s, Routes routes, __nv_bfloat16* out) {
+  __shared__ float weights[32];
+  __shared__ unsigned has;
+  const int token = blockIdx.x, column = (blockIdx.y * kMixThreads + threadIdx.x) * 4;
+  if (threadIdx.x < 32) {
+    const int pair = token * L.K + threadIdx.x;
+    const bool valid = static_cast<int>(threadIdx.x) < L.K && routes.expert(pair, L.K, L.E) >= 0;
+    weights[threadIdx.x] = valid ? routes.weight(pair) : 0.0f;
+    const unsigned mask = __ballot_sync(kFull, valid);
+    if (threadIdx.x == 0) has = mask;
+  }
+  __syncthreads();
   grid_dependency_wait();
   grid_dependency_release();
-  const int token = blockIdx.x, column = (blockIdx.y * kMixThreads + threadIdx.x) * 8;
   if (column >= L.H) return;
-  float sum[8] = {};
-  for (int k = 0; k < L.K; ++k) {
-    const int pair = token * L.K + k;
-    if (routes.expert(pair, L.K, L.E) < 0) continue;
-    const float w = routes.weight(pair);
-    const float4* from = reinterpret_cast<const float4*>(s.sums + static_cast<size_t>(pair) * L.H + column);
-    const float4 a = from[0], b = from[1];
-    const float v[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+  const float* from = s.sums + static_cast<size_t>(token) * L.K * L.H + column;
+  float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  for (int first = 0; first < L.K; first += kMixAhead) {
+    float4 v[kMixAhead];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) sum[i] = __fmaf_rn(w, v[i], sum[i]);
-  }
-  uint32_t words[4];
+    for (int k = 0; k < kMixAhead; ++k)
+      if (has >> (first + k) & 1) v[k] = *reinterpret_cast<const float4*>(from + static_cast<size_t>(first + k) * L.H);
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const __nv_bfloat162 pair = __floats2bfloat162_rn(sum[2 * i], sum[2 * i + 1]);
-    words[i] = *reinterpret_cast<const uint32_t*>(&pair);
+    for (int k = 0; k < kMixAhead; ++k) {
+      if (!(has >> (first + k) & 1)) continue;
+      const float w = weights[first + k];
+      sum = make_float4(__fmaf_rn(w, v[k].x, sum.x), __fmaf_rn(w, v[k].y, sum.y), __fmaf_rn(w, v[k].z, sum.z),
+                        __fmaf_rn(w, v[k].w, sum.w));
+    }
   }
-  *reinterpret_cast<uint4*>(out + static_cast<size_t>(token) * L.H + column) =
-      make_uint4(words[0], words[1], words[2], words[3]);
+  const __nv_bfloat162 lo = __floats2bfloat162_rn(sum.x, sum.y), hi = __floats2bfloat162_rn(sum.z, sum.w);
+  *reinterpret_cast<uint2*>(out + static_cast<size_t>(token) * L.H + column) =
+      make_uint2(*reinterpret_cast<const uint32_t*>(&lo), *reinterpret_cast<const uint32_t*>(&hi));
 }
 
 // ---- host ------------------------------------------------------------------------------------------
@@ -577,13 +604,15 @@ int cfm_experts_forward(const cfm_experts* layer, void* workspace, int32_t capac
   const int busy = static_cast<int>(std::min<int64_t>(L.E, pairs));
   auto* out = static_cast<__nv_bfloat16*>(call->out);
   if (pairs <= kFewPairs) return run_few(L, s, routes, hidden, busy, out, st);
+  if (const int code = allow_everything<k_group_pairs>(false)) return code;
   const int pass = pass_pairs(pairs, busy);
-  launch_dependent(k_group_pairs, dim3(1), dim3(kGroupThreads), sizeof(int) * L.E, st, routes, L.E, L.K, pass, s);
+  launch_dependent(k_group_pairs, dim3(1), dim3(kGroupThreads), sizeof(int) * (L.E + kGroupKept * kGroupThreads), st,
+                   routes, L.E, L.K, pass, s);
   const int code = pass == 32   ? run_tensor<32>(L, s, hidden, pairs, st)
                    : pass == 64 ? run_tensor<64>(L, s, hidden, pairs, st)
                                 : run_tensor<144>(L, s, hidden, pairs, st);
   if (code) return code;
-  launch_dependent(k_experts_mix, dim3(call->tokens, (L.H + 8 * kMixThreads - 1) / (8 * kMixThreads)), dim3(kMixThreads), 0,
+  launch_dependent(k_experts_mix, dim3(call->tokens, (L.H + 4 * kMixThreads - 1) / (4 * kMixThreads)), dim3(kMixThreads), 0,
                    st, L, s, routes, out);
   return launched();
 }

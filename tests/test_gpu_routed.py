@@ -239,6 +239,19 @@ def test_weights_beyond_32_bits_of_elements():
         assert torch.equal(got, want) and got.any()
 
 
+@pytest.mark.parametrize("tokens,experts,top_k", [(1024, 12, 8), (1100, 40, 8), (300, 4096, 32), (9000, 3, 1)])
+def test_more_pairs_than_the_grouping_keeps(tokens, experts, top_k):
+    """Up to 8192 pairs are put in order in shared memory; each token as in a call of its own."""
+    gate_up, down = layer(128, 16, experts)
+    x, ids, weights = batch(tokens, 128, experts, top_k)
+    out = RoutedExperts(gate_up, down, top_k, tokens)(x, ids, weights)
+    part = RoutedExperts(gate_up, down, top_k, 50)
+    for start in (0, tokens // 2, tokens - 50):
+        rows = slice(start, start + 50)
+        assert torch.equal(out[rows], part(x[rows], ids[rows], weights[rows]))
+    check(gate_up, down, x[-40:], ids[-40:], weights[-40:])
+
+
 def test_as_an_opaque_operator():
     from cfm_b200.runtime import ops
 
