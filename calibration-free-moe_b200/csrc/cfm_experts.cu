@@ -117,9 +117,13 @@ __global__ void __launch_bounds__(kGroupThreads) k_group_pairs(Routes routes, in
 #pragma unroll
   for (int j = 0; j < kGroupKept; ++j)
     if (expert[j] >= 0) rank[j] = atomicAdd(&count[expert[j]], 1);
-  for (int p = tid + kGroupKept * kGroupThreads; p < pairs; p += kGroupThreads) {
-    const int e = routes.expert(p, K, E);
-    if (e >= 0) atomicAdd(&count[e], 1);
+  const bool fits = pairs <= kGroupKept * kGroupThreads;
+  if (!fits) {
+    __syncthreads();  // the places are among the pairs kept
+    for (int p = tid + kGroupKept * kGroupThreads; p < pairs; p += kGroupThreads) {
+      const int e = routes.expert(p, K, E);
+      if (e >= 0) atomicAdd(&count[e], 1);
+    }
   }
   __syncthreads();
   // Pairs and passes before those of this thread, in one number.
@@ -157,7 +161,6 @@ __global__ void __launch_bounds__(kGroupThreads) k_group_pairs(Routes routes, in
   }
   if (tid == 0) s.counts[0] = static_cast<int>(warps[31] >> kPassBits);
   __syncthreads();
-  const bool fits = pairs <= kGroupKept * kGroupThreads;
 #pragma unroll
   for (int j = 0; j < kGroupKept; ++j) {
     if (expert[j] < 0) continue;
