@@ -9,9 +9,8 @@
 //   mix     router weights, sum over a token's slots in their order, BF16
 // up and down are cfm_experts_tc.cuh's; calls of few pairs have two kernels of their own, without lists.
 // Sums are FP32.  The tensor cores take the type of the weights, so an activation goes to them as two BF16
-// terms, its value rounded and what that leaves: 2^-17 of it is lost, and of the output's error of 2^-9 nothing is theirs.
-// (Rounded once to BF16 they would have added as much as the output's own rounding: 0.0024 of the output's norm
-// instead of 0.0016.)
+// terms, its value rounded and what that leaves: at most 2^-16 of it is lost, beside the 2^-8 of the output's rounding.
+// (Rounded once to BF16 they would have added as much as that: 0.0024 of the output's norm instead of 0.0016.)
 // A pair's numbers do not depend on its place in the list nor on the other pairs: a token's output does not depend
 // on the tokens beside it, but for calls of few pairs, whose kernels add in another order.
 #include "cfm_device.cuh"

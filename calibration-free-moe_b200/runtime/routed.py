@@ -33,8 +33,8 @@ class RoutedWorkspace:
         self.bytes = _native.load().cfm_experts_workspace_bytes(ctypes.byref(layer), capacity)
         if self.bytes < 0:
             raise ValueError(_native.load().cfm_error_string(self.bytes).decode())
-        self.buffer = torch.zeros(self.bytes, device=device, dtype=torch.uint8)
-        self.status = self.buffer[:4].view(torch.int32)
+        self.buffer = torch.empty(self.bytes, device=device, dtype=torch.uint8)
+        self.status = self.buffer[:4].view(torch.int32).zero_()
 
 
 class RoutedExperts:
@@ -78,7 +78,7 @@ class RoutedExperts:
             workspace = RoutedWorkspace(hidden, width, experts, top_k, max_tokens, gate_up.device)
         if (
             workspace.key != (hidden, width, experts, top_k)
-            or workspace.capacity < max_tokens
+            or not 1 <= max_tokens <= workspace.capacity
             or workspace.buffer.device != gate_up.device
         ):
             raise ValueError("Shared workspace must match the layer's dimensions and device")

@@ -463,17 +463,18 @@ typedef struct cfm_experts {
   const void* down;       /* bf16 physical [E, I, H] (channel-major)           */
 } cfm_experts;
 
-/* Scratch bytes for calls of up to `capacity` tokens, fewer than 2^24 pairs (a host computation; negative: a CFM_E_*
- * code).  The caller zeroes the scratch once; one call at a time may use it.  Its first int32 is
- * a status: not zero if a wait inside a kernel ran out (after about a second), when the
- * outputs of that call are not to be trusted. */
+/* Scratch bytes for calls of up to `capacity` tokens, fewer than 2^24 pairs (a host computation;
+ * negative: a CFM_E_* code).  On a 16-byte boundary; one call at a time may use it.  Its first
+ * int32 is a status, which the caller zeroes once: not zero if a wait inside a kernel ran out
+ * (after about a second), when the outputs of that call are not to be trusted. */
 int64_t cfm_experts_workspace_bytes(const cfm_experts* layer, int32_t capacity);
 
 /* out[t] = sum over slots k of weights[t, k] D_e (phi(G_e x_t) * (U_e x_t)), e = ids[t, k], all
  * channels.  Of `call`: tokens, ids, weights, padding, hidden, out and the two type flags, as
- * cfm_reader_forward takes them; hidden, out and the weights on 16-byte boundaries.  An id outside of [0, E) adds nothing; a token may have an expert
- * more than once.  Padding rows read nothing and produce zero rows.  Sums are FP32, activations keep
- * 16 bits, the output is rounded once.  A token's bits do not depend on the other tokens, except
+ * cfm_reader_forward takes them; hidden, out and the weights on 16-byte boundaries.  An id
+ * outside of [0, E) adds nothing; a token may have an expert more than once.  Padding rows read
+ * nothing and produce zero rows.  Sums are FP32, activations keep 16 bits, the output is rounded
+ * once.  A token's bits do not depend on the other tokens, except
  * between calls of up to 16 (token, slot) pairs and larger ones. */
 int cfm_experts_forward(const cfm_experts* layer, void* workspace, int32_t capacity,
                         const cfm_call* call, void* stream);

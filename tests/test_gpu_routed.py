@@ -341,6 +341,8 @@ def test_refusals():
         RoutedExperts(gate_up, down, 2, 8, workspace=RoutedWorkspace(256, 48, 4, 3, 8, "cuda"))
     with pytest.raises(ValueError):
         RoutedExperts(gate_up, down, 2, 8, workspace=RoutedWorkspace(256, 48, 4, 2, 7, "cuda"))
+    with pytest.raises(ValueError):
+        RoutedExperts(gate_up, down, 2, 0, workspace=RoutedWorkspace(256, 48, 4, 2, 7, "cuda"))
     run = RoutedExperts(gate_up, down, 2, 8)
     x, ids, weights = batch(8, 256, 4, 2)
     for call in (
