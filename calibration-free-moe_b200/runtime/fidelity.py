@@ -48,13 +48,13 @@ def token_logprobs(logits: Tensor, tokens: Tensor, top: int = 0) -> TokenScores:
     if not 0 <= top <= MAX_TOP or top > struct.columns:
         raise ValueError(f"top must be from 0 to {MAX_TOP} and at most the vocabulary's size")
     logprobs = logits.new_empty(rows, dtype=torch.float32)
-    entropy = logits.new_empty(rows, dtype=torch.float32)
+    entropy = torch.empty_like(logprobs)
     if not top:
         enqueue("cfm_token_logprobs", index, byref(struct), tokens.data_ptr(), wide, 0,
                 logprobs.data_ptr(), entropy.data_ptr(), None, None)
         return TokenScores(logprobs, entropy, None, None)
-    top_ids = logits.new_empty((rows, top), dtype=torch.int32)
-    top_logprobs = logits.new_empty((rows, top), dtype=torch.float32)
+    top_logprobs = logprobs.new_empty((rows, top))
+    top_ids = torch.empty_like(top_logprobs, dtype=torch.int32)
     enqueue("cfm_token_logprobs", index, byref(struct), tokens.data_ptr(), wide, top,
             logprobs.data_ptr(), entropy.data_ptr(), top_ids.data_ptr(), top_logprobs.data_ptr())
     return TokenScores(logprobs, entropy, top_ids, top_logprobs)
@@ -80,7 +80,7 @@ def compare_logits(reference: Tensor, logits: Tensor) -> tuple[Tensor, Tensor]:
     ):
         raise ValueError("Both rows of logits must have one shape, type and device")
     divergence = logits.new_empty(rows, dtype=torch.float32)
-    agreement = logits.new_empty(rows, dtype=torch.bool)
+    agreement = torch.empty_like(divergence, dtype=torch.bool)
     enqueue("cfm_compare_logits", index, byref(one), byref(other), divergence.data_ptr(),
             agreement.data_ptr())
     return divergence, agreement

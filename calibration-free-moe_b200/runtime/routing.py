@@ -39,7 +39,7 @@ def route_tokens(
     if ids_dtype not in (torch.int32, torch.int64):
         raise ValueError("Expert ids are int32 or int64")
     weights = logits.new_empty((rows, top_k), dtype=weights_dtype)
-    ids = logits.new_empty((rows, top_k), dtype=ids_dtype)
+    ids = torch.empty_like(weights, dtype=ids_dtype)
     enqueue("cfm_route_tokens", logits.get_device(), byref(struct), top_k, renormalize,
             ids.data_ptr(), ids_dtype is torch.int64, weights.data_ptr(),
             weights_dtype is torch.bfloat16)
