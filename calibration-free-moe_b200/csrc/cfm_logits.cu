@@ -622,7 +622,7 @@ constexpr int kCompareChunks = 2;  // that are on their way or looked at
 constexpr int kCompareChunk = kComparePieces * kScoreThreads;
 constexpr size_t kCompareRing = 2ull * kCompareChunks * kComparePieces * kScoreThreads * 16;  // of two rows
 constexpr float kSlack = 2.0f;     // by which an a may be above its exponential's shift
-constexpr float kNear = 60.0f;     // |t| of the single pass; beyond, and where a row has -inf alone, NaN or +inf, there is another
+constexpr float kNear = 60.0f;     // |t| and shifts of the single pass; beyond, and where a row has -inf alone, NaN or +inf, there is another
 
 // psi(t) / t^2 for |t| up to 1/2: the series to t^6, whose last term the Chebyshev polynomial of degree six turns into
 // lower ones; 3e-8 of the value.
@@ -842,6 +842,8 @@ __global__ void __launch_bounds__(kScoreThreads, kScorePerSm)
         }
       }
       d = __shfl_sync(kFull, d, __ffs(__ballot_sync(kFull, top_a == chunk)) - 1);
+      // Banned by b, or t would lose what x and y have beside the rows' distance.
+      if (!(fabsf(d) <= kNear)) sum.beyond = 1;
       if (sum.m > -kInfinity) {
         const float f = exp_fast(__fsub_rn(sum.m, chunk));
         reshift(sum, d);

@@ -1,0 +1,75 @@
+"""Divergence of logits where rows are masked, far apart or of unusual size, against 64 bits.
+
+Where tolerances come from, with SUM and STEP as in test_gpu_logits.py.  t is the difference of a pair of logits less
+that at the reference's largest, and is off by a few steps of the numbers that it is made of: x, y as they stand where
+the rows are at most 60 apart there, else x and y less their values there.  A psi(t) = e^-t - 1 + t is off by 2^-22 of t^2
+or of |t| + 1 and by what t is off, a sum by SUM of its terms' sizes, and where KL is E[t] + log E[e^-t] the logarithm
+by SUM / E[e^-t] of them, E[e^-t] 1/64 at least (else it has a sum of its own).
+"""
+
+import math
+
+import pytest
+import torch
+
+import cfm_b200  # noqa: F401
+from cfm_b200.runtime.fidelity import compare_logits
+from test_gpu_logits import STEP, SUM, TYPES, logits, ranked
+
+pytestmark = pytest.mark.gpu
+
+INF, NAN = math.inf, math.nan
+
+
+def in_64_bits(a, b):
+    """KL(softmax(a) || softmax(b)), and how far from it the library may be."""
+    x, y = a.double(), b.double()
+    top = x.amax(-1, keepdim=True)
+    none = ~(top.isfinite() & y.amax(-1, keepdim=True).isfinite())
+    log_p, log_q = torch.log_softmax(x, -1), torch.log_softmax(y, -1)
+    p, q = log_p.exp(), log_q.exp()
+    gap = torch.where(p > 0, log_p - log_q, 0.0)
+    # With q - p added to each term, whose sum is zero.
+    near = gap.abs() < 1
+    terms = torch.where(near, p * (gap + torch.expm1(-gap.clamp(-1, 1))), p * gap - p + q)
+    want = torch.where(none, NAN, torch.where(p > 0, terms, q).sum(-1, keepdim=True))[:, 0]
+    at = ranked(a, 1)
+    u, v = x - top, y - y.gather(1, at)
+    apart = (top - y.gather(1, at)).abs()
+    t = u - v
+    own = torch.minimum((x - y).abs(), torch.full_like(apart, 120.0))
+    off = STEP * torch.where(t.abs() < 0.5, t.abs(), 2.0) * (own + u.abs() + v.abs() + t.abs())
+    size = torch.where(t.abs() < 0.5, t.square(), t.abs() + 1.0)
+    live = (p > 0) & t.isfinite()
+    allowed = torch.where(live, p * (2 * SUM * size + 4 * off), 0.0).sum(-1)
+    far = (torch.where(live, p * size, 0.0).sum(-1) > 0.25) | ((p == 0) & (q > 0)).any(-1)
+    return want, allowed + 4 * SUM * want + torch.where(far & (want > 0.1), 2 * SUM, 0.0)
+
+
+def check(a, b):
+    divergence, agreement = compare_logits(a, b)
+    assert torch.equal(agreement, ranked(a, 1)[:, 0] == ranked(b, 1)[:, 0])
+    want, allowed = in_64_bits(a, b)
+    same = (divergence.double() == want) | (divergence.isnan() & want.isnan())
+    off = torch.where(same, 0.0, (divergence.double() - want).abs())
+    assert (off <= allowed.nan_to_num(0.0, 0.0, 0.0)).all(), (divergence, want, allowed)
+    return divergence
+
+
+def pair(rows, vocabulary, dtype, noise=0.1, seed=None):
+    a = logits(rows, vocabulary, torch.float32, rows + vocabulary if seed is None else seed)
+    generator = torch.Generator(device="cuda").manual_seed(vocabulary)
+    b = a + noise * torch.randn(a.shape, device="cuda", generator=generator)
+    return a.to(dtype), b.to(dtype)
+
+
+# -- rows banned altogether ------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("vocabulary", [8, 1000, 8192, 32768, 131072, 262144])
+@pytest.mark.parametrize("rows", [1, 32, 256])
+def test_rows_banned_altogether(dtype, vocabulary, rows):
+    """A vocabulary that fills every chunk, or not."""
+    a, b = pair(rows, vocabulary, dtype)
+    banned = torch.full_like(a, -INF)
+    for x, y in ((a, banned), (banned, b), (banned, banned)):
+        assert check(x, y).isnan().all()
