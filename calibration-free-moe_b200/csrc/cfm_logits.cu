@@ -854,7 +854,9 @@ __global__ void __launch_bounds__(kScoreThreads, kScorePerSm)
       sum.shift = d;
       sum.m = chunk;
     }
-    if (fabsf(sum.m) <= kModerate) {
+    if (!(fabsf(sum.m) <= kModerate)) {
+      if (top_b != -kInfinity) sum.beyond = 1;  // Q has something where P has had nothing yet
+    } else {
       const float m = sum.m, shift = sum.shift;
       const float c = __fmul_rn(m, kLog2E), back = exp2_fast(-__fmaf_rn(m, kLog2E, -c));
       const Pair scale = pair_of(kLog2E, kLog2E), base = pair_of(-c, -c), minus = pair_of(-1.0f, -1.0f), less = pair_of(-shift, -shift);

@@ -73,3 +73,34 @@ def test_rows_banned_altogether(dtype, vocabulary, rows):
     banned = torch.full_like(a, -INF)
     for x, y in ((a, banned), (banned, b), (banned, banned)):
         assert check(x, y).isnan().all()
+
+
+# -- tokens that the reference alone bans ------------------------------------------------------
+BANS = [(1024, 512, 1024), (1024, 510, 1024), (512, 0, 256), (8192, 4096, 8192), (8192, 2048, 6144), (20000, 0, 10000),
+        (131072, 0, 65536), (131072, 65536, 131072), (50257, 4096, 50257), (50257, 0, 50000), (3000, 128, 256)]
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("vocabulary,start,end", BANS)
+@pytest.mark.parametrize("rows", [1, 9, 64])
+def test_blocks_that_the_reference_alone_bans(dtype, vocabulary, start, end, rows):
+    a, b = pair(rows, vocabulary, dtype)
+    a[:, start:end] = -INF
+    assert check(a, b).isfinite().all()
+    flat = torch.zeros_like(a)
+    check(torch.where(a == -INF, a, flat), flat)
+    b[0, start + (end - start) // 2] = INF
+    assert check(a, b)[0].isnan()
+    b[0, start + (end - start) // 2] = NAN
+    assert check(a, b)[0].isnan()
+    b[:, start:end] = -INF  # both do
+    assert check(a, b).isfinite().all()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("vocabulary", [8, 1000, 32768, 262144])
+def test_rows_with_one_token_left(dtype, vocabulary):
+    a, b = pair(9, vocabulary, dtype)
+    banned = torch.full_like(a, -INF)
+    banned[:, 3] = 1.0
+    assert (check(a, banned) == INF).all() and check(banned, b).isfinite().all()
