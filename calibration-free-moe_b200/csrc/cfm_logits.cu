@@ -22,6 +22,8 @@ constexpr float kLog2E = 1.44269504f;
 constexpr float kInfinity = __builtin_huge_valf();
 // Stands for -inf where sums want a finite number: beside a largest value of up to kModerate its exponential is zero.
 constexpr float kLeast = -1e30f, kModerate = 1e29f;
+// Largest size of a shift m for which m log2 e may be rounded: by half a unit of the last place, 1 at most.
+constexpr float kScaled = 16777216.0f;
 
 // 2^x, two units in the last place; 0 below -126.
 __device__ __forceinline__ float exp2_fast(float x) {
@@ -452,7 +454,7 @@ __global__ void __launch_bounds__(kScoreThreads, kScorePerSm)
       m = chunk;
     }
     if (m == -kInfinity) continue;  // nothing but -inf so far
-    if (fabsf(m) <= kModerate) {
+    if (fabsf(m) <= kScaled) {
       // In powers of two, from one multiply-add per element: 2^t, t = x log2 e - c, c = m log2 e as it rounds.
       // m itself has t = t_m, next to zero; with that the chunk's sums are brought to the shift m.
       const float c = __fmul_rn(m, kLog2E), t_m = __fmaf_rn(m, kLog2E, -c);
@@ -488,10 +490,12 @@ __global__ void __launch_bounds__(kScoreThreads, kScorePerSm)
       weighted = __fmaf_rn(0.693147181f * back, (w0 + w1) - t_m * all, weighted);
       continue;
     }
-#pragma unroll 1
-    for (int p = first + tid; p < min(end, first + kChunk); p += kScoreThreads) {  // values beyond 10^29, or NaN, which the shift tells of
+    // Larger ones (a mask of a finite value, mostly), or NaN, which the shift tells of.  (The same as above with m taken from the
+    // elements first, by a test per piece: 39.2 us for 512 rows of 151936, against 38.4.)
+#pragma unroll
+    for (int j = 0; j < kScorePieces; ++j) {
       float x[W];
-      E::widen(row.load(p), x);
+      E::widen(v[j], x);
 #pragma unroll
       for (int i = 0; i < W; ++i) {
         const float d = x[i] == m ? kLeast : fmaxf(__fsub_rn(x[i], m), kLeast);  // -inf: adds nothing
