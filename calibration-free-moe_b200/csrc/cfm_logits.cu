@@ -724,6 +724,30 @@ __device__ __noinline__ ulonglong2 largest_of_chunks(Row<T> a, Row<T> b, int2 fi
   return make_ulonglong2(place[0] < 0x7fffffff ? placed(value.x, place[0]) : 0, place[1] < 0x7fffffff ? placed(value.y, place[1]) : 0);
 }
 
+// The single pass over a thread's pieces of a chunk whose exponentials' shift is larger than kScaled: a mask of a finite
+// value, mostly.  `from`: its first slot.  Mass, mean, rest and the largest |t|.
+template <typename T>
+__device__ __noinline__ float4 large_moments(uint32_t ring, int from, float m, float shift) {
+  using E = Element<T>;
+  constexpr int W = E::kWidth;
+  float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 1
+  for (int j = 0; j < kComparePieces; ++j) {
+    float x[W], y[W];
+    E::widen_bounded(load_shared16(ring_slot(ring, from + j)), x);
+    E::widen_bounded(load_shared16(ring_slot(ring, from + kComparePieces + j)), y);
+#pragma unroll
+    for (int i = 0; i < W; ++i) {
+      const float e = exp_fast(__fsub_rn(x[i], m)), t = __fsub_rn(__fsub_rn(x[i], y[i]), shift);
+      sum.x += e;
+      sum.y = __fmaf_rn(e, t, sum.y);
+      sum.z = __fmaf_rn(e, psi(t), sum.z);
+      sum.w = fmaxf(sum.w, fabsf(t));
+    }
+  }
+  return sum;
+}
+
 // The other pass, over rows that are far apart or have -inf where the other has not: sums of e^(a - max a), of that
 // times t and, with `apart`, of e^(b - max b); else of e^(a - max a) psi(t), where an element of which P has nothing
 // adds its e^(b - b*), for the sum of all of those is Q's.  `infinite`: Q has nothing where P has something.
@@ -860,6 +884,12 @@ __global__ void __launch_bounds__(kScoreThreads, kScorePerSm)
     }
     if (!(fabsf(sum.m) <= kModerate)) {
       if (top_b != -kInfinity) sum.beyond = 1;  // Q has something where P has had nothing yet
+    } else if (fabsf(sum.m) > kScaled) {
+      const float4 more = large_moments<T>(ring, slot, sum.m, sum.shift);
+      sum.mass += more.x;
+      sum.mean += more.y;
+      sum.rest += more.z;
+      if (!(more.w <= kNear)) sum.beyond = 1;
     } else {
       const float m = sum.m, shift = sum.shift;
       const float c = __fmul_rn(m, kLog2E), back = exp2_fast(-__fmaf_rn(m, kLog2E, -c));

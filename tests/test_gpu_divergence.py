@@ -104,3 +104,27 @@ def test_rows_with_one_token_left(dtype, vocabulary):
     banned = torch.full_like(a, -INF)
     banned[:, 3] = 1.0
     assert (check(a, banned) == INF).all() and check(banned, b).isfinite().all()
+
+
+# -- finite values of any size -----------------------------------------------------------------
+LARGE = [-1e4, -1e7, -1e8, -1e9, -3e9, -1e10, -1e11, -1e12, -1e15, -1e20, -1e25, -1e28, -3e29, -1e31]
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("fill", LARGE)
+def test_rows_masked_by_a_finite_value(dtype, fill):
+    for rows, vocabulary, start, end in ((3, 8192, 0, 6000), (260, 8192, 0, 6000), (2, 50257, 0, 40000), (2, 1024, 0, 512), (5, 70000, 30000, 70000)):
+        a, b = pair(rows, vocabulary, dtype)
+        a[:, start:end] = b[:, start:end] = fill
+        assert check(a, b).isfinite().all()
+    a[:, :] = b[:, :] = fill  # nothing else
+    assert not check(a, b).any()
+    a[:, 77] = b[:, 77] = -fill
+    assert not check(a, b).any()
+    a, b = pair(4, 5000, dtype)
+    a[:, 100], b[:, 100] = -fill, -fill
+    assert not check(a, b).any()
+    a, b = pair(4, 5000, dtype)
+    a[:, 2000:] = fill
+    b[:, 2000:] = 2 * fill
+    check(a, b)
