@@ -1002,7 +1002,8 @@ __global__ void __launch_bounds__(kScoreThreads, kScorePerSm)
     top_a = warp_max(of.tops[0]);
     top_b = warp_max(of.tops[1]);
     if (lane == 0) {
-      s_beyond = all.beyond;
+      // Shifts that add up may have taken the sums beyond FP32.
+      s_beyond = all.beyond || !(all.mass > 0.0f && fabsf(all.mean) < kInfinity && fabsf(all.rest) < kInfinity);
       tops[0][0] = top_a;
       tops[1][0] = top_b;
     }

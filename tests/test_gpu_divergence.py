@@ -128,3 +128,18 @@ def test_rows_masked_by_a_finite_value(dtype, fill):
     a[:, 2000:] = fill
     b[:, 2000:] = 2 * fill
     check(a, b)
+
+
+# -- steps of the shift ------------------------------------------------------------------------
+def test_shifts_that_add_up():
+    """Chunks whose differences are 59 apart from the next one's."""
+    for far in (30.0, 45.0, 59.0):
+        a = torch.zeros((256, 4096), device="cuda")
+        b = torch.zeros_like(a)
+        b[:, :2048] = far
+        for i in range(2):
+            a[:, 2048 * i:2048 * (i + 1):128] = 3.0 * i + 1
+            b[:, 2048 * i:2048 * (i + 1):128] = 3.0 * i + 1 - far * i
+        check(a, b)
+        check(a[:5], b[:5])
+        check(a.flip(-1), b.flip(-1))
