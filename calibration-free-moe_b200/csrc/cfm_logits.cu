@@ -748,38 +748,49 @@ __device__ __noinline__ float4 large_moments(uint32_t ring, int from, float m, f
   return sum;
 }
 
-// The other pass, over rows that are far apart or have -inf where the other has not: sums of e^(a - max a), of that
-// times t and, with `apart`, of e^(b - max b); else of e^(a - max a) psi(t), where an element of which P has nothing
-// adds its e^(b - b*), for the sum of all of those is Q's.  `infinite`: Q has nothing where P has something.
+// Sums of the other pass: of e = e^(a - max a), of e t, of e psi(t) and of e^(b - b*), which is e e^-t and all of Q; whether
+// Q has nothing where P has something.  In 64 bits, as a thread adds up to a thousand times.
+struct FarMoments {
+  double mass, mean, rest, other;
+  int infinite;
+};
+
+// The other pass, over rows that are far apart or have -inf where the other has not.  What Q has where P has nothing adds
+// to the rest as it is.
 template <typename T>
-__device__ __noinline__ Moments far_moments(Row<T> a, Row<T> b, int begin, int end, float most_a, float base_b,
-                                            bool apart) {
+__device__ __noinline__ FarMoments far_moments(Row<T> a, Row<T> b, int begin, int end, float most_a, float base_b) {
   using E = Element<T>;
   constexpr int W = E::kWidth;
-  Moments sum = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0};
+  FarMoments sum = {0.0, 0.0, 0.0, 0.0, 0};
   const float shift = most_a - base_b;
 #pragma unroll 1
   for (int p = begin + threadIdx.x; p < end; p += kScoreThreads) {
-    float x[W], y[W];
+    float x[W], y[W], mass = 0.0f, mean = 0.0f, rest = 0.0f, other = 0.0f;
     E::widen(a.load(p), x);
     E::widen(b.load(p), y);
 #pragma unroll
     for (int i = 0; i < W; ++i) {
       const float t = __fsub_rn(__fsub_rn(x[i], y[i]), shift), size = fabsf(t);
       const float e = x[i] > -kInfinity ? exp_fast(__fsub_rn(x[i], most_a)) : 0.0f;
-      if (x[i] > -kInfinity && y[i] == -kInfinity) sum.beyond = 1;
+      if (x[i] > -kInfinity && y[i] == -kInfinity) sum.infinite = 1;
       const float u = e > 0.0f ? __fmul_rn(e, t) : 0.0f, of_b = exp_fast(__fsub_rn(y[i], base_b));
-      sum.mass += e;
-      sum.mean += u;
-      sum.rest += apart ? of_b : size <= 16.0f ? __fmul_rn(e, psi(t)) : of_b - e + u;
+      mass += e;
+      mean += u;
+      other += of_b;
+      rest += size <= 16.0f ? __fmul_rn(e, psi(t)) : of_b - e + u;
     }
+    sum.mass += mass;
+    sum.mean += mean;
+    sum.rest += rest;
+    sum.other += other;
   }
 #pragma unroll
   for (int w = 16; w; w >>= 1) {
     sum.mass += __shfl_xor_sync(kFull, sum.mass, w);
     sum.mean += __shfl_xor_sync(kFull, sum.mean, w);
     sum.rest += __shfl_xor_sync(kFull, sum.rest, w);
-    sum.beyond |= __shfl_xor_sync(kFull, sum.beyond, w);
+    sum.other += __shfl_xor_sync(kFull, sum.other, w);
+    sum.infinite |= __shfl_xor_sync(kFull, sum.infinite, w);
   }
   return sum;
 }
@@ -795,6 +806,7 @@ __global__ void __launch_bounds__(kScoreThreads, kScorePerSm)
   extern __shared__ __align__(16) uint8_t compare_shared[];
   __shared__ Compared compared;
   __shared__ Moments moments[kScoreWarps];
+  __shared__ FarMoments far[kScoreWarps];
   __shared__ u64 tops[2][kScoreWarps];
   __shared__ float highs[2][kScoreWarps];
   __shared__ int s_beyond;
@@ -1018,33 +1030,32 @@ __global__ void __launch_bounds__(kScoreThreads, kScorePerSm)
   } else {
     const float most_a = value_of(static_cast<uint32_t>(tops[0][0] >> 32)), most_b = value_of(static_cast<uint32_t>(tops[1][0] >> 32));
     const float b_there = E::one(b.data + place_of(tops[0][0]));
-    // Rows without a distribution (nothing but -inf, with NaN or with +inf); rows so far apart that e^(b - b*) overflows.
+    // Rows without a distribution (nothing but -inf, with NaN or with +inf); rows so far apart that e^(b - b*) overflows,
+    // of which b's largest is b*.
     const bool none = !(fabsf(most_a) < kInfinity) || !(fabsf(most_b) < kInfinity), apart = !(most_b - b_there <= kNear);
-    sum = {};
-    if (!none) sum = far_moments(a, b, begin, end, most_a, apart ? most_b : b_there, apart);
-    cluster_meet();  // all have read the first ones
-    if (lane == 0) moments[warp] = sum;
+    FarMoments mine = {};
+    if (!none) mine = far_moments(a, b, begin, end, most_a, apart ? most_b : b_there);
+    if (lane == 0) far[warp] = mine;
     __syncthreads();
     cluster_meet();
     if (rank == 0 && warp == 0) {
-      double mass_of = 0.0, mean_of = 0.0, rest_of = 0.0;
-      int infinite = 0;
+      FarMoments total = {};
       for (int i = 0; i < ranks * kScoreWarps; ++i) {
-        const Moments of = *of_rank(&moments[i % kScoreWarps], i / kScoreWarps);
-        mass_of += of.mass;
-        mean_of += of.mean;
-        rest_of += of.rest;
-        infinite |= of.beyond;
+        const FarMoments of = *of_rank(&far[i % kScoreWarps], i / kScoreWarps);
+        total.mass += of.mass;
+        total.mean += of.mean;
+        total.rest += of.rest;
+        total.other += of.other;
+        total.infinite |= of.infinite;
       }
+      const double mean_of = total.mean / total.mass, rest_of = total.rest / total.mass, x = rest_of - mean_of;
       if (none) {
         kl = __longlong_as_double(0x7fffffffffffffffll);
-      } else if (infinite) {
+      } else if (total.infinite) {
         kl = kInfinity;
-      } else if (apart) {
-        kl = mean_of / mass_of + log(rest_of / mass_of);
       } else {
-        const double remainder = rest_of / mass_of, x = remainder - mean_of / mass_of;
-        kl = fabs(x) < 0.5 ? remainder + (log1p(x) - x) : mean_of / mass_of + log1p(x);
+        // E[|t|] is below E[psi] + 1: where that is large, 1 + x is lost in the difference, and has a sum of its own.
+        kl = rest_of < 1.0 && fabs(x) < 0.5 ? rest_of + (log1p(x) - x) : mean_of + log(total.other / total.mass);
       }
     }
   }

@@ -143,3 +143,15 @@ def test_shifts_that_add_up():
         check(a, b)
         check(a[:5], b[:5])
         check(a.flip(-1), b.flip(-1))
+
+
+# -- distances of any size ----------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("fill", [-1e4, -1e7, -1e10, -1e15, -1e20])
+def test_what_only_the_other_row_masks(dtype, fill):
+    """A divergence of the mask's size."""
+    for rows, vocabulary, start, end in ((3, 8192, 0, 6000), (260, 8192, 2000, 8192), (2, 50257, 5000, 5001)):
+        a, b = pair(rows, vocabulary, dtype)
+        b[:, start:end] = fill
+        check(a, b)
+        check(torch.zeros_like(a), torch.where(b == fill, b, torch.zeros_like(b)))
