@@ -649,10 +649,18 @@ struct Moments {
   int beyond;
 };
 
-// The same of another shift of t.
-__device__ __forceinline__ void reshift(Moments& s, float shift) {
+// What the single pass has of E[e^-t] = 1 + E[psi] - E[t], Q's part, times the mass: a difference.
+__device__ __forceinline__ float other_of(const Moments& s) { return s.mass + (s.rest - s.mean); }
+// Where it is small (Q is sure of a token, and t large for all others), its digits are lost: at 1/64 six bits of them.
+constexpr float kLeastOther = 1.0f / 64.0f;
+// A larger t makes e^-t smaller: of a large one the difference then keeps only what the digits have left, 2^-24 of it.
+constexpr float kMostOther = 256.0f;
+
+// The same of another shift of t.  mass, other: of all that are to be moved alike.
+__device__ __forceinline__ void reshift(Moments& s, float shift, float mass, float other) {
   const float by = __fsub_rn(s.shift, shift);
-  if (!(fabsf(by) <= kNear)) s.beyond = 1;
+  if (!(fabsf(by) <= kNear && (by >= 0.0f || other >= kLeastOther * mass) && (by <= 0.0f || other <= kMostOther * mass)))
+    s.beyond = 1;
   const float more = psi(by), less = fabsf(by) <= 0.5f ? __fsub_rn(more, by) : exp_fast(-by) - 1.0f;  // e^-by - 1
   s.rest = s.rest + (less * (s.rest - s.mean) + more * s.mass);
   s.mean = __fmaf_rn(by, s.mass, s.mean);
@@ -668,7 +676,7 @@ __device__ __noinline__ Moments moments_of_lanes(Moments s) {
   const bool has = s.mass > 0.0f;
   const unsigned having = __ballot_sync(kFull, has && s.m == m);
   const float shift = __shfl_sync(kFull, s.shift, having ? __ffs(having) - 1 : 0);
-  if (has) reshift(s, shift);
+  if (has) reshift(s, shift, s.mass, other_of(s));
   const float f = has ? exp_fast(__fsub_rn(s.m, m)) : 0.0f;
   Moments all;
   all.m = m;
@@ -886,7 +894,13 @@ __global__ void __launch_bounds__(kScoreThreads, kScorePerSm)
       if (!(fabsf(d) <= kNear)) sum.beyond = 1;
       if (sum.m > -kInfinity) {
         const float f = exp_fast(__fsub_rn(sum.m, chunk));
-        reshift(sum, d);
+        float mass = sum.mass, other = other_of(sum);  // the warp's
+#pragma unroll
+        for (int w = 16; w; w >>= 1) {
+          mass += __shfl_xor_sync(kFull, mass, w);
+          other += __shfl_xor_sync(kFull, other, w);
+        }
+        reshift(sum, d, mass, other);
         sum.mass *= f;
         sum.mean *= f;
         sum.rest *= f;
@@ -1015,7 +1029,8 @@ __global__ void __launch_bounds__(kScoreThreads, kScorePerSm)
     top_b = warp_max(of.tops[1]);
     if (lane == 0) {
       // Shifts that add up may have taken the sums beyond FP32.
-      s_beyond = all.beyond || !(all.mass > 0.0f && fabsf(all.mean) < kInfinity && fabsf(all.rest) < kInfinity);
+      s_beyond = all.beyond || !(all.mass > 0.0f && fabsf(all.mean) < kInfinity && fabsf(all.rest) < kInfinity &&
+                                 other_of(all) >= kLeastOther * all.mass);
       tops[0][0] = top_a;
       tops[1][0] = top_b;
     }

@@ -145,6 +145,22 @@ def test_shifts_that_add_up():
         check(a.flip(-1), b.flip(-1))
 
 
+# -- a flat reference and a token that the other is sure of ------------------------------------
+@pytest.mark.parametrize("vocabulary", [64, 1000, 8192, 50257])
+@pytest.mark.parametrize("rise", [2.0, 5.0, 12.0, 30.0, 50.0, 59.0, 80.0])
+def test_flat_reference_and_a_sure_row(vocabulary, rise):
+    generator = torch.Generator(device="cuda").manual_seed(vocabulary)
+    a = 0.01 * torch.randn((40, vocabulary), device="cuda", generator=generator)
+    b = a + 0.01 * torch.randn(a.shape, device="cuda", generator=generator)
+    places = torch.randint(0, vocabulary, (40, 1), device="cuda", generator=generator)
+    places[::2] = a[::2].argmax(-1, keepdim=True)
+    for many in (1, 20):
+        b.scatter_(1, (places + torch.arange(many, device="cuda") * 37) % vocabulary, rise)
+        check(a, b)
+        check(b, a)
+        check(a, -b)
+
+
 # -- distances of any size ----------------------------------------------------------------------
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 @pytest.mark.parametrize("fill", [-1e4, -1e7, -1e10, -1e15, -1e20])
