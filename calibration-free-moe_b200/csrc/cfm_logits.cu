@@ -770,7 +770,6 @@ __device__ __noinline__ FarMoments far_moments(Row<T> a, Row<T> b, int begin, in
   using E = Element<T>;
   constexpr int W = E::kWidth;
   FarMoments sum = {0.0, 0.0, 0.0, 0.0, 0};
-  const float shift = most_a - base_b;
 #pragma unroll 1
   for (int p = begin + threadIdx.x; p < end; p += kScoreThreads) {
     float x[W], y[W], mass = 0.0f, mean = 0.0f, rest = 0.0f, other = 0.0f;
@@ -778,10 +777,12 @@ __device__ __noinline__ FarMoments far_moments(Row<T> a, Row<T> b, int begin, in
     E::widen(b.load(p), y);
 #pragma unroll
     for (int i = 0; i < W; ++i) {
-      const float t = __fsub_rn(__fsub_rn(x[i], y[i]), shift), size = fabsf(t);
-      const float e = x[i] > -kInfinity ? exp_fast(__fsub_rn(x[i], most_a)) : 0.0f;
+      // Not (x - y) less a shift: where the rows are far apart, x - y has lost what x and y have beside that.
+      const float below = __fsub_rn(x[i], most_a), below_b = __fsub_rn(y[i], base_b);
+      const float t = __fsub_rn(below, below_b), size = fabsf(t);
+      const float e = exp_fast(below), of_b = exp_fast(below_b);
       if (x[i] > -kInfinity && y[i] == -kInfinity) sum.infinite = 1;
-      const float u = e > 0.0f ? __fmul_rn(e, t) : 0.0f, of_b = exp_fast(__fsub_rn(y[i], base_b));
+      const float u = e > 0.0f ? __fmul_rn(e, t) : 0.0f;
       mass += e;
       mean += u;
       other += of_b;

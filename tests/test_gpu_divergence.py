@@ -161,6 +161,30 @@ def test_flat_reference_and_a_sure_row(vocabulary, rise):
         check(a, -b)
 
 
+# -- rows a constant apart ---------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("offset", [50.0, 100.0, 1e3, 2e4, 1e6, 1e8])
+def test_rows_a_constant_apart(dtype, offset):
+    if dtype == torch.float16 and offset > 6e4:
+        offset = 6e4
+    for sign in (1.0, -1.0):
+        a, b = pair(5, 9000, torch.float32, 0.5)
+        b = (b + sign * offset).to(dtype)
+        check(a.to(dtype), b)
+        check(b, a.to(dtype))
+        check(a.to(dtype), torch.full_like(b, sign * offset))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("fill", LARGE)
+def test_a_reference_masked_by_a_finite_value_in_part_and_altogether(dtype, fill):
+    a, b = pair(4, 5000, dtype)
+    a[:, 2000:] = fill
+    check(a, b)
+    a[:, :2000] = fill
+    check(a, b)
+
+
 # -- distances of any size ----------------------------------------------------------------------
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 @pytest.mark.parametrize("fill", [-1e4, -1e7, -1e10, -1e15, -1e20])
