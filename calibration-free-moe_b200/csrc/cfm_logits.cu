@@ -756,6 +756,7 @@ __device__ __noinline__ float4 large_moments(uint32_t ring, int from, float m, f
   return sum;
 }
 
+constexpr float kWeight = -745.0f;  // the logarithm of the least weight beside the largest, e^-745: what 64 bits hold
 // Sums of the other pass: of e = e^(a - max a), of e t, of e psi(t) and of e^(b - b*), which is e e^-t and all of Q; whether
 // Q has nothing where P has something.  In 64 bits, as a thread adds up to a thousand times.
 struct FarMoments {
@@ -781,7 +782,7 @@ __device__ __noinline__ FarMoments far_moments(Row<T> a, Row<T> b, int begin, in
       const float below = __fsub_rn(x[i], most_a), below_b = __fsub_rn(y[i], base_b);
       const float t = __fsub_rn(below, below_b), size = fabsf(t);
       const float e = exp_fast(below), of_b = exp_fast(below_b);
-      if (x[i] > -kInfinity && y[i] == -kInfinity) sum.infinite = 1;
+      if (below >= kWeight && y[i] == -kInfinity) sum.infinite = 1;
       const float u = e > 0.0f ? __fmul_rn(e, t) : 0.0f;
       mass += e;
       mean += u;

@@ -67,9 +67,9 @@ def compare_logits(reference: Tensor, logits: Tensor) -> tuple[Tensor, Tensor]:
     distance; T may be zero.  Returns the divergence in nats (FP32 `[T]`) and a bool `[T]`: the
     largest logits of the two rows are at the same token, equal ones by the lowest id.  Rows that
     hardly differ keep their digits: no sums of the size of the logits are subtracted.  The
-    divergence is +inf where the reference gives weight to a token that `logits` bans, and NaN
-    where a row has NaN or +inf or is banned altogether.  Enqueued on the current stream; no
-    gradients.
+    divergence is +inf where the reference gives weight to a token that `logits` bans (e^-745 of its
+    largest weight at least: not where it masks by a finite value), and NaN where a row has NaN or
+    +inf or is banned altogether.  Enqueued on the current stream; no gradients.
     """
     one, _ = check_rows(reference, "Reference logits", MAX_VOCABULARY)
     other, rows = check_rows(logits, "Logits", MAX_VOCABULARY)

@@ -446,8 +446,8 @@ int cfm_token_logprobs(const cfm_rows* logits, const void* tokens, int32_t token
 
 /* Two sets of rows of one shape and type: KL(softmax(reference) || softmax(logits)) of each
  * pair in nats, and whether the largest logits are at the same place (ties as above).  +inf
- * where the reference gives weight to what the other gives none; NaN where either has no
- * distribution. */
+ * where the reference gives weight (e^-745 of its largest at least, so not where it masks by a
+ * finite value) to what the other gives none; NaN where either has no distribution. */
 int cfm_compare_logits(const cfm_rows* reference, const cfm_rows* logits, float* divergence,
                        uint8_t* agreement, void* stream);
 

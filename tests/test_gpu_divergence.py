@@ -195,3 +195,18 @@ def test_what_only_the_other_row_masks(dtype, fill):
         b[:, start:end] = fill
         check(a, b)
         check(torch.zeros_like(a), torch.where(b == fill, b, torch.zeros_like(b)))
+
+
+# -- weights that are none ---------------------------------------------------------------------
+@pytest.mark.parametrize("vocabulary", [16, 4096, 20000])
+def test_a_banned_token_of_no_weight(vocabulary):
+    """A reference that masks by a finite value what the other bans: no weight that 64 bits hold is lost."""
+    for dtype in TYPES:
+        a, b = pair(6, vocabulary, dtype)
+        a[:, 5:12] = torch.finfo(dtype).min
+        b[:, 5:12] = -INF
+        divergence = check(a, b)
+        assert divergence.isfinite().all()
+        a[3, 5], a[4, 7] = -800.0, -700.0
+        divergence = check(a, b)
+        assert divergence[3].isfinite() and divergence[4] == INF
