@@ -756,8 +756,9 @@ __device__ __noinline__ float4 large_moments(uint32_t ring, int from, float m, f
   return sum;
 }
 
+constexpr float kPart = 1.0f / 16.0f;
 constexpr float kWeight = -745.0f;  // the logarithm of the least weight beside the largest, e^-745: what 64 bits hold
-// Sums of the other pass: of e = e^(a - max a), of e t, of e psi(t) and of e^(b - b*), which is e e^-t and all of Q; whether
+// Sums of the other pass: of e = e^(a - max a), of e t times kPart, of e psi(t) and of e^(b - b*), which is e e^-t and all of Q; whether
 // Q has nothing where P has something.  In 64 bits, as a thread adds up to a thousand times.
 struct FarMoments {
   double mass, mean, rest, other;
@@ -778,14 +779,21 @@ __device__ __noinline__ FarMoments far_moments(Row<T> a, Row<T> b, int begin, in
     E::widen(b.load(p), y);
 #pragma unroll
     for (int i = 0; i < W; ++i) {
-      // Not (x - y) less a shift: where the rows are far apart, x - y has lost what x and y have beside that.
-      const float below = __fsub_rn(x[i], most_a), below_b = __fsub_rn(y[i], base_b);
-      const float t = __fsub_rn(below, below_b), size = fabsf(t);
-      const float e = exp_fast(below), of_b = exp_fast(below_b);
-      if (below >= kWeight && y[i] == -kInfinity) sum.infinite = 1;
+      // Not (x - y) less a shift: where the rows are far apart, x - y has lost what x and y have beside that.  In
+      // sixteenths, so that differences of the largest numbers and a piece's sum of them are finite.
+      const float below = __fsub_rn(kPart * x[i], kPart * most_a), below_b = __fsub_rn(kPart * y[i], kPart * base_b);
+      const float part = __fsub_rn(below, below_b), t = part / kPart, size = fabsf(t);
+      const float e = exp_fast(below / kPart), of_b = exp_fast(below_b / kPart);
+      const bool given = below >= kPart * kWeight;
+      if (given && y[i] == -kInfinity) sum.infinite = 1;
+      if (given && e == 0.0f) {  // t may be larger than e is small
+        const double more = exp(static_cast<double>(below) / kPart) * part;
+        sum.mean += more;
+        sum.rest += more / kPart;
+      }
       const float u = e > 0.0f ? __fmul_rn(e, t) : 0.0f;
       mass += e;
-      mean += u;
+      mean += e > 0.0f ? __fmul_rn(e, part) : 0.0f;
       other += of_b;
       rest += size <= 16.0f ? __fmul_rn(e, psi(t)) : of_b - e + u;
     }
@@ -1065,7 +1073,7 @@ __global__ void __launch_bounds__(kScoreThreads, kScorePerSm)
         total.other += of.other;
         total.infinite |= of.infinite;
       }
-      const double mean_of = total.mean / total.mass, rest_of = total.rest / total.mass, x = rest_of - mean_of;
+      const double mean_of = total.mean / (kPart * total.mass), rest_of = total.rest / total.mass, x = rest_of - mean_of;
       if (none) {
         kl = __longlong_as_double(0x7fffffffffffffffll);
       } else if (total.infinite) {

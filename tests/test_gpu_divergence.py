@@ -50,7 +50,8 @@ def check(a, b):
     divergence, agreement = compare_logits(a, b)
     assert torch.equal(agreement, ranked(a, 1)[:, 0] == ranked(b, 1)[:, 0])
     want, allowed = in_64_bits(a, b)
-    same = (divergence.double() == want) | (divergence.isnan() & want.isnan())
+    # Beyond FP32's numbers, as rounded to it: infinite.
+    same = (divergence == want.float()) | (divergence.isnan() & want.isnan())
     off = torch.where(same, 0.0, (divergence.double() - want).abs())
     assert (off <= allowed.nan_to_num(0.0, 0.0, 0.0)).all(), (divergence, want, allowed)
     return divergence
@@ -210,3 +211,24 @@ def test_a_banned_token_of_no_weight(vocabulary):
         a[3, 5], a[4, 7] = -800.0, -700.0
         divergence = check(a, b)
         assert divergence[3].isfinite() and divergence[4] == INF
+
+
+# -- the largest numbers -----------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("vocabulary", [9, 4096, 20000])
+def test_the_other_row_masks_by_its_types_lowest_value(dtype, vocabulary):
+    """Divergences as large as the type's numbers, of which some sum to more, and of next to no weight."""
+    most = torch.finfo(dtype).max
+    a, b = pair(5, vocabulary, dtype)
+    b[:, 2:9] = -most
+    check(a, b)
+    check(torch.zeros_like(a), b)
+    a[:, 2:9] = -100.0
+    check(a, b)
+    a[:, 2:9] = -most
+    assert check(a, b).isfinite().all()
+    a, b = pair(5, vocabulary, dtype)
+    b[:, 3], b[:, 4] = most, -most
+    a[:, 4] = 9.0
+    check(a, b)
+    check(b, a)
