@@ -206,35 +206,33 @@ constexpr int kFewPairs = 16;
 struct Few {
   int e;          // expert, -1: there are fewer
   unsigned mask;  // its pairs
-  bool twice;     // some token has it twice
 };
 // Of a warp, a pair per lane.
 struct FewGroups {
   int e;           // the lane's expert
   unsigned same;   // lanes with that expert
   unsigned first;  // the first lane of every busy expert
-  unsigned again;  // lanes of the same token with that expert
 
   __device__ FewGroups(const Routes& routes, int K, int E) {
     const int lane = threadIdx.x & 31;
     e = lane < routes.tokens * K ? routes.expert(lane, K, E) : -1;
     same = __match_any_sync(kFull, e);
     first = __ballot_sync(kFull, e >= 0 && lane == __ffs(same) - 1);
-    again = same & __match_any_sync(kFull, lane / K) & ~(1u << lane);
   }
   __device__ int experts() const { return __popc(first); }
   // The `which`-th busy expert, in the order of first pairs.
   __device__ Few group(int which) const {
-    if (which >= experts()) return {-1, 0, false};
+    if (which >= experts()) return {-1, 0};
     unsigned rest = first;
     for (int i = 0; i < which; ++i) rest &= rest - 1;
     const int from = __ffs(rest) - 1;
     Few few;
     few.e = __shfl_sync(kFull, e, from);
     few.mask = __shfl_sync(kFull, same, from);
-    few.twice = __any_sync(kFull, e == few.e && again);
     return few;
   }
+  // The place of the lane's expert among the busy ones, -1 where it has none.
+  __device__ int which() const { return e < 0 ? -1 : __popc(first & ((1u << (__ffs(same) - 1)) - 1)); }
 };
 // The pair at a place among the set bits, -1 behind them.
 __device__ __forceinline__ int pair_at(unsigned mask, int place) {
@@ -344,24 +342,29 @@ constexpr int kFewDownColumns = 64;  // of a cluster
 constexpr int kFewDownAhead = 4;     // steps of 16 channels whose rows are on their way
 constexpr int kFewRanks = 8;         // CTAs of a cluster
 
-// grid (8 H / 64): a cluster has 64 outputs of all tokens, its CTAs share the experts, or where those are few
-// their channels; a CTA's warps share a CTA's channels.  A thread has 16 bytes, eight outputs, of four channels'
+// grid (8 H / 64): a cluster has 64 outputs of all pairs, its CTAs share the experts, of which each has SPLITS parts of the
+// channels; a CTA's warps share a part.  A thread has 16 bytes, eight outputs, of four channels'
 // rows; the first operand's registers pair two channels of one output, which two byte permutations per pair of
 // words do.  The first rows are on their way before the kernel before this one has ended.
-// Sums of warps and of CTAs are added in their order.
+// A token's bits do not depend on the tokens beside it: a pair's warps and parts are added in their order, a token's pairs in
+// that of its slots.  So the parts go by K, not by how many experts a call has.
+template <int SPLITS>
 __global__ void __launch_bounds__(kFewDownThreads, 2)
     k_few_down(Experts L, Scratch s, Routes routes, __nv_bfloat16* out) {
   __shared__ float parts[kFewDownWarps][8][kFewDownColumns];
-  __shared__ float total[kFewPairs][kFewDownColumns];
+  __shared__ float total[kFewPairs][kFewDownColumns];  // of a pair, the channels of this CTA
+  __shared__ float weights[kFewPairs];
+  __shared__ int units[kFewPairs];  // a pair's first unit, -1: it has no expert
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
   const int rank = blockIdx.x % kFewRanks, h0 = blockIdx.x / kFewRanks * kFewDownColumns;
-  for (int i = tid; i < routes.tokens * kFewDownColumns; i += kFewDownThreads) total[0][i] = 0.0f;
   const FewGroups groups(routes, L.K, L.E);
-  const int experts = groups.experts(), splits = experts >= 5 ? 1 : experts >= 3 ? 2 : experts == 2 ? 4 : 8;
+  const int experts = groups.experts();
+  const float weight = tid < kFewPairs && groups.e >= 0 ? routes.weight(tid) : 0.0f;
+  if (tid < kFewPairs) units[tid] = groups.e >= 0 ? groups.which() * SPLITS : -1;
   bool waited = false;
-  for (int unit = rank; unit < experts * splits; unit += kFewRanks) {
-    const Few few = groups.group(unit / splits);
-    const int count = __popc(few.mask), part = unit % splits * kFewDownWarps + warp, pieces = splits * kFewDownWarps;
+  for (int unit = rank; unit < experts * SPLITS; unit += kFewRanks) {
+    const Few few = groups.group(unit / SPLITS);
+    const int count = __popc(few.mask), part = unit % SPLITS * kFewDownWarps + warp, pieces = SPLITS * kFewDownWarps;
     const int begin = L.I / 16 * part / pieces, end = L.I / 16 * (part + 1) / pieces;
     const __nv_bfloat16* rows = L.down + (static_cast<size_t>(few.e) * L.I + 4 * t) * L.H + h0 + 8 * g;
     for (int pass = 0; pass < count; pass += 8) {
@@ -410,32 +413,43 @@ __global__ void __launch_bounds__(kFewDownThreads, 2)
         to[1] = make_float4(acc[2][c], acc[2][2 + c], acc[3][c], acc[3][2 + c]);
       }
       __syncthreads();
-      // A token that has this expert twice: its pairs are added one after another.
-      const int tokens = min(8, count - pass), together = few.twice ? 1 : tokens;
-      for (int from = 0; from < tokens; from += together) {
-        for (int i = tid; i < together * kFewDownColumns; i += kFewDownThreads) {
-          const int token = from + i / kFewDownColumns, column = i % kFewDownColumns;
-          float sum = parts[0][token][column];
+      for (int i = tid; i < min(8, count - pass) * kFewDownColumns; i += kFewDownThreads) {
+        const int place = i / kFewDownColumns, column = i % kFewDownColumns;
+        float sum = parts[0][place][column];
 #pragma unroll
-          for (int j = 1; j < kFewDownWarps; ++j) sum += parts[j][token][column];
-          const int of = pair_at(few.mask, pass + token);
-          float& to = total[of / L.K][column];
-          to = __fmaf_rn(routes.weight(of), sum, to);
-        }
-        if (few.twice) __syncthreads();
+        for (int j = 1; j < kFewDownWarps; ++j) sum += parts[j][place][column];
+        total[pair_at(few.mask, pass + place)][column] = sum;
       }
     }
   }
   if (!waited) grid_dependency_wait();
   grid_dependency_release();
+  if (tid < kFewPairs) weights[tid] = weight;
   __syncthreads();
   cluster_meet();
   constexpr int kShare = kFewDownColumns / kFewRanks;
   for (int i = tid; i < routes.tokens * kShare; i += kFewDownThreads) {
     const int token = i / kShare, column = rank * kShare + i % kShare;
     float sum = 0.0f;
+    constexpr int kSlots = kFewRanks / SPLITS;  // whose parts are on their way together
+    for (int from = 0; from < L.K; from += kSlots) {
+      float v[kSlots][SPLITS];
 #pragma unroll
-    for (int j = 0; j < kFewRanks; ++j) sum += *of_rank(&total[token][column], j);
+      for (int j = 0; j < kSlots; ++j) {
+        const int pair = token * L.K + from + j, unit = from + j < L.K ? units[pair] : -1;
+#pragma unroll
+        for (int part = 0; part < SPLITS; ++part)
+          v[j][part] = unit >= 0 ? *of_rank(&total[pair][column], (unit + part) % kFewRanks) : 0.0f;
+      }
+#pragma unroll
+      for (int j = 0; j < kSlots; ++j) {
+        const int pair = token * L.K + from + j;
+        if (from + j >= L.K || units[pair] < 0) continue;
+#pragma unroll
+        for (int part = 1; part < SPLITS; ++part) v[j][0] += v[j][part];
+        sum = __fmaf_rn(weights[pair], v[j][0], sum);
+      }
+    }
     out[static_cast<size_t>(token) * L.H + h0 + column] = __float2bfloat16_rn(sum);
   }
   cluster_meet();  // the others' shared memory has been read
@@ -522,8 +536,11 @@ int run_few(const Experts& L, const Scratch& s, const Routes& routes, const __nv
             __nv_bfloat16* out, cudaStream_t stream) {
   const int64_t items = static_cast<int64_t>(busy) * (L.I / 8);
   launch_dependent(k_few_up, dim3(static_cast<unsigned>(std::min<int64_t>(items, 148 * kFewUpPerSm))), dim3(kFewUpThreads), 0, stream, L, s, routes, hidden);
-  launch_clusters(k_few_down, dim3(L.H / kFewDownColumns * kFewRanks), dim3(kFewDownThreads), 0, kFewRanks, stream, L, s,
-                  routes, out);
+  // Parts of an expert's channels.  One, two and four of them, us of a call: K = 1 of 16 experts of width 1024, one token 13.9, 11.6, 11.4,
+  // 16 tokens 34.2, 33.5, 37.3; K = 2 of 8 of hidden 4096 and width 1408, one token 34.0, 26.4, 23.9, eight tokens 61.4, 64.2, 68.8;
+  // K = 4 of 16 of width 512, one token 13.0, 12.5 (two), four tokens 20.6, 21.8.
+  const auto down = L.K >= 3 ? k_few_down<1> : k_few_down<2>;
+  launch_clusters(down, dim3(L.H / kFewDownColumns * kFewRanks), dim3(kFewDownThreads), 0, kFewRanks, stream, L, s, routes, out);
   return launched();
 }
 
