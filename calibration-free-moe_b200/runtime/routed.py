@@ -168,14 +168,17 @@ class RoutedExperts:
             _native.check(code, "cfm_experts_forward")
 
     def check_status(self) -> None:
-        """Raise if a wait inside a kernel of this workspace's calls ran out (they end after a
-        second); that call's rows are not to be trusted.  Synchronises with the device."""
+        """Raise if a wait inside a kernel ran out (they end after a second) in a call that used this
+        workspace since the last report; the rows of those calls, of any layer that shares it, are
+        not to be trusted.  Reporting clears the status.  Synchronises with the device."""
         if int(self.workspace.status):
+            self.workspace.status.zero_()
             raise RuntimeError("routed-expert kernels reported a device-side error")
 
     def rows(self, x: Tensor, topk_weights: Tensor, topk_ids: Tensor) -> Tensor:
         """Any number of rows, in calls of at most `max_tokens`: the stock callable of
-        `ProgressiveExperts`."""
+        `ProgressiveExperts`.  As with its reader, the program calls `check_status` where it
+        synchronises anyway; nothing here does."""
         x, ids, weights = x.contiguous(), topk_ids.contiguous(), topk_weights.contiguous()
         out = torch.empty_like(x)
         for start in range(0, x.shape[0], self.max_tokens):
