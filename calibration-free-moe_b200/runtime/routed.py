@@ -170,7 +170,8 @@ class RoutedExperts:
     def check_status(self) -> None:
         """Raise if a wait inside a kernel ran out (they end after a second) in a call that used this
         workspace since the last report; the rows of those calls, of any layer that shares it, are
-        not to be trusted.  Reporting clears the status.  Synchronises with the device."""
+        not to be trusted.  Reporting clears the status.  Waits for the device, whatever the stream."""
+        torch.cuda.synchronize(self._device)
         if int(self.workspace.status):
             self.workspace.status.zero_()
             raise RuntimeError("routed-expert kernels reported a device-side error")

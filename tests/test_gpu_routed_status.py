@@ -26,3 +26,16 @@ def test_a_report_clears_the_status(tokens):
         run.check_status()
         run(x, ids, weights)
         run.check_status()
+
+
+def test_a_call_on_another_stream_is_waited_for():
+    workspace = RoutedWorkspace(256, 48, 4, 2, 32, "cuda")
+    run = RoutedExperts(*layer(256, 48, 4), 2, 32, workspace=workspace)
+    torch.cuda.synchronize()
+    stream = torch.cuda.Stream()
+    with torch.cuda.stream(stream):
+        torch.cuda._sleep(50_000_000)  # some 25 ms
+        workspace.status.fill_(1)
+    with pytest.raises(RuntimeError, match="device-side"):
+        run.check_status()
+    run.check_status()
