@@ -16,6 +16,7 @@ from torch import Tensor
 
 from .. import _native
 from ..activation import ACTIVATION_CODES, GatedActivation
+from .rows import wants_gradient
 
 
 class RoutedWorkspace:
@@ -106,6 +107,8 @@ class RoutedExperts:
         experts adds nothing.  Writes `[T, H]` into `out` (allocated if None; it may not overlap the
         other arguments) on the current stream.
         """
+        if wants_gradient(hidden) or wants_gradient(weights):
+            raise ValueError("Routed input requires grad: this operator has no derivative")
         tokens = hidden.shape[0] if hidden.ndim == 2 else 0
         device = self._device
         if (
@@ -144,8 +147,6 @@ class RoutedExperts:
             )
         ):
             raise ValueError("Routed input exceeds the prepared token/expert contract")
-        if (hidden.requires_grad or weights.requires_grad) and torch.is_grad_enabled():
-            raise ValueError("Routed input requires grad: this operator has no backward pass")
         if out is None:
             out = torch.empty_like(hidden)
         call = _native.Call(

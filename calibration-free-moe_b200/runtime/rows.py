@@ -7,10 +7,18 @@ from functools import cache
 
 import torch
 from torch import Tensor
+from torch.autograd import forward_ad
 
 from .. import _native
 
 TYPE_CODES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
+
+
+def wants_gradient(tensor: Tensor) -> bool:
+    """Whether autograd would follow an operation on it, backward or forward."""
+    return (tensor.requires_grad and torch.is_grad_enabled()) or (
+        forward_ad._current_level >= 0 and forward_ad.unpack_dual(tensor).tangent is not None
+    )
 
 
 def check_rows(logits: Tensor, what: str, most_columns: int) -> tuple[_native.Rows, int]:
@@ -26,8 +34,8 @@ def check_rows(logits: Tensor, what: str, most_columns: int) -> tuple[_native.Ro
     step, one = logits.stride()
     if (one != 1 and columns > 1) or (step < columns and rows > 1):
         raise ValueError(f"{what} must have contiguous rows that do not overlap")
-    if logits.requires_grad and torch.is_grad_enabled():
-        raise ValueError(f"{what} requires grad: this operator has no backward pass")
+    if wants_gradient(logits):
+        raise ValueError(f"{what} requires grad: this operator has no derivative")
     return _native.Rows(logits.data_ptr(), step, rows, columns, code), rows
 
 
