@@ -669,6 +669,22 @@ __device__ __forceinline__ void reshift(Moments& s, float shift, float mass, flo
   s.shift = shift;
 }
 
+// A warp's moments with the shifts m of the exponentials and `shift` of t, the same in all lanes.
+__device__ __noinline__ Moments moved(Moments s, float m, float shift) {
+  float mass = s.mass, other = other_of(s);  // the warp's
+#pragma unroll
+  for (int w = 16; w; w >>= 1) {
+    mass += __shfl_xor_sync(kFull, mass, w);
+    other += __shfl_xor_sync(kFull, other, w);
+  }
+  reshift(s, shift, mass, other);
+  const float f = exp_fast(__fsub_rn(s.m, m));
+  s.mass *= f;
+  s.mean *= f;
+  s.rest *= f;
+  return s;
+}
+
 // The lanes' moments as one, in every lane, with the shift of a lane that has the largest a: where nearly all of the
 // mass is on one element, t is zero there, and the small parts of the others are not lost beside it.
 __device__ __noinline__ Moments moments_of_lanes(Moments s) {
@@ -904,19 +920,7 @@ __global__ void __launch_bounds__(kScoreThreads, kScorePerSm)
       d = __shfl_sync(kFull, d, __ffs(__ballot_sync(kFull, top_a == chunk)) - 1);
       // Banned by b, or t would lose what x and y have beside the rows' distance.
       if (!(fabsf(d) <= kNear)) sum.beyond = 1;
-      if (sum.m > -kInfinity) {
-        const float f = exp_fast(__fsub_rn(sum.m, chunk));
-        float mass = sum.mass, other = other_of(sum);  // the warp's
-#pragma unroll
-        for (int w = 16; w; w >>= 1) {
-          mass += __shfl_xor_sync(kFull, mass, w);
-          other += __shfl_xor_sync(kFull, other, w);
-        }
-        reshift(sum, d, mass, other);
-        sum.mass *= f;
-        sum.mean *= f;
-        sum.rest *= f;
-      }
+      if (sum.m > -kInfinity) sum = moved(sum, chunk, d);
       sum.shift = d;
       sum.m = chunk;
     }
