@@ -197,7 +197,7 @@ __global__ void __launch_bounds__(kGroupThreads) k_group_pairs(Routes routes, in
 }
 
 // ---- few pairs -------------------------------------------------------------------------------------
-// Calls of up to 16 pairs in two launches (two tokens of the 128-expert layer 36 us, 43 on the tensor-core path; three 50
+// Calls of up to 16 pairs in two launches (two tokens of the 128-expert layer 35 us, 43 on the tensor-core path; three would take 50
 // and 50, four 65 and 62).  The weights go from global memory straight into the registers of
 // warp-level tensor-core products (m16n8k16), whose eight columns are the tokens of an expert.  Every warp
 // groups the pairs by itself, a pair per lane.
@@ -565,10 +565,10 @@ int make_map(CUtensorMap* map, const void* data, int64_t rows, int64_t columns) 
 }
 
 // Pairs of a pass, for `busy` experts.  A second pass over an expert reads its weights again, from L2; a stage with room for
-// more tokens leaves fewer stages in the ring.  Passes of 16, 32, 64 and 128, us of a call: 64 tokens of the
-// 128-expert layer (4 per expert) 200, 195, 196, 205; 256 of 256 experts with a skewed router (8) 192, 168, 168, 169.  Of 128, 144,
-// 160 and 192: 400 of 64 experts of width 768 (50) 145, 141, 150, 151; 1000 of 64 experts of width 1024 (125) 275, 267, 261, 263;
-// 1000 of 32 experts of hidden 1024 (250) 129, 121, 131, 142.
+// more tokens leaves fewer stages in the ring.  us of a call, measured in turn at the clocks of a busy GPU, of passes of 16, 32, 64 and 128:
+// 64 tokens of the 128-expert layer (4 per expert) 203, 198, 204, 213; 256 of 256 experts with a skewed router (8) 209, 177, 175, 181.  Of 64,
+// 128, 144, 160 and 192: 400 of 64 experts of width 768 (50) 136, 141, 141, 141, 150; 1000 of 64 experts of width 1024 (125) 364, 272, 236,
+// 226, 239; 3000 of those (375) 934, 604, 616, 663, 629; 1000 of 32 experts of hidden 1024 (250) 162, 149, 135, 140, 154.
 int pass_pairs(int64_t pairs, int64_t busy) { return pairs <= 12 * busy ? 32 : pairs <= 40 * busy ? 64 : 144; }
 
 template <int TOKENS>

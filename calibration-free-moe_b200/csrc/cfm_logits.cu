@@ -622,7 +622,9 @@ __global__ void __launch_bounds__(kScoreThreads, kScorePerSm)
 // psi(t) = e^-t - 1 + t and x = E[psi] - E[t], it is
 //   E[psi] + (log1p(x) - x),
 // where nothing of first order in t is left to cancel: rows that hardly differ keep their digits in FP32.
-// A shift is changed by D without loss: psi(t + D) = e^-D psi(t) + psi(D) - (e^-D - 1) t.
+// A shift is changed by D: psi(t + D) = e^-D psi(t) + psi(D) - (e^-D - 1) t.
+// 1 + x = E[e^-t] is a difference, whose digits t must not be large for; rows of which it has too few left take another pass, with a
+// sum of its own for it: E[t] + log E[e^-t].  (128 rows of 131072 FP32 99 us with the other pass, 30 without.)
 constexpr int kComparePieces = 2;  // of a thread and row that are looked at together
 constexpr int kCompareChunks = 2;  // that are on their way or looked at
 constexpr int kCompareChunk = kComparePieces * kScoreThreads;
@@ -903,8 +905,8 @@ __global__ void __launch_bounds__(kScoreThreads, kScorePerSm)
     }
     const float chunk = warp_max_nan(top_a);
     // Too large to be scaled, or NaN.
-    if ((!(fabsf(chunk) <= kModerate) && chunk != -kInfinity) || top_b != top_b) sum.beyond = 1;
-    if (chunk > sum.m + kSlack && chunk <= kModerate) {  // new shifts, the same in the whole warp: of its largest a
+    if (!(chunk <= kModerate) || top_b != top_b) sum.beyond = 1;
+    if (chunk > sum.m + kSlack && fabsf(chunk) <= kModerate) {  // new shifts, the same in the whole warp: of its largest a
       float d = 0.0f;
       if (top_a == chunk) {
 #pragma unroll 1
@@ -925,7 +927,8 @@ __global__ void __launch_bounds__(kScoreThreads, kScorePerSm)
       sum.m = chunk;
     }
     if (!(fabsf(sum.m) <= kModerate)) {
-      if (top_b != -kInfinity) sum.beyond = 1;  // Q has something where P has had nothing yet
+      // P has had nothing yet: -inf, or a mask that leaves no weight beside any logit of moderate size.  If Q has ...
+      if (!(top_b < -kModerate)) sum.beyond = 1;
     } else if (fabsf(sum.m) > kScaled) {
       const float4 more = large_moments<T>(ring, slot, sum.m, sum.shift);
       sum.mass += more.x;
@@ -1114,9 +1117,12 @@ static int check_rows(const cfm_rows* rows, int most_columns) {
 }
 
 // CTAs that share a row: until the call has 256, more than one for most SMs, or a thread has one piece.  What a CTA does after its
-// sums (5 to 8 us with top alternatives, all latency) grows with their number.  Log probabilities of 151936 BF16 logits,
-// us of 1, 2, 4, 8 and 16 CTAs per row: one row 14.5, 10.0, 7.3, 4.7, 4.2; 128 rows 15.1, 13.9, 15.1, 17.3; 512 rows 38.6, 38.3,
-// 48, 54, with 20 alternatives 63, 74, 102, 114.
+// sums (5 to 8 us with top alternatives, all latency) grows with their number.  us of 1, 2, 4, 8 and 16 CTAs per row of 151936 BF16 logits,
+// log probabilities: one row 14.5, 9.4, 6.9, 5.6, 4.0; 32 rows 14.8, 9.7, 8.1, 8.0, 8.5; 128 rows 15.8, 13.8, 15.2, 20.5, 24.5; 300 rows
+// 34.7, 26.7, 30.2, 40.9, 53.6; 600 rows 43.0, 43.5, 53.6; 512 rows with 20 alternatives 63, 74, 102, 114.  Divergence: one row 32.7, 20.2,
+// 14.0, 10.8, 9.4; 32 rows 34.4, 21.1, 16.1, 14.6, 21.6; 128 rows 35.4, 29.4, 31.0, 39.9, 63.1; 300 rows 83, 60, 64, 82; 600 rows 104, 99, 115.
+// So from 256 to some 500 rows of such length two CTAs would be faster than the one taken; for short rows they are slower (300 rows of 8192:
+// 6.2 and 8.1, 12.1 and 15.4; of 32003: 12.9 and 12.5, 30.7 and 29.7).
 static int row_ranks(int rows, int columns, int type) {
   const int pieces = columns / (16 / element_bytes(type)) + 1;
   int ranks = 1;
